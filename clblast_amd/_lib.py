@@ -27,6 +27,9 @@ class Double2(ctypes.Structure):
     _fields_ = [("x", ctypes.c_double), ("y", ctypes.c_double)]
 
 
+LAYER_ROUTINES = ["gemmEpilogue", "gemmActivationGradient", "activationGradient", "gemmGrouped", "gemmGroupedGradient"]
+
+
 def _declare(lib):
     sz, vp = c_size_t, c_void_p
     for prefix, scalar, real in (("C", Float2, c_float), ("Z", Double2, c_double)):
@@ -63,6 +66,21 @@ def _declare(lib):
         f.argtypes = [c_int, c_int, c_int, sz, sz, sz, scalar, vp, sz, sz, sz, vp, sz, sz, sz, scalar, vp, sz, sz, sz,
                       sz, vp, vp]
         f.restype = c_int
+    for prefix in "SHB":  # the layer products: fp32, fp16 and bf16 data, scalars as floats
+        groups = [sz, vp, sz]
+        layer = {
+            "gemmEpilogue": [c_int, c_int, sz, sz, sz, c_float, vp, sz, sz, vp, sz, sz, vp, sz, c_int, vp, sz, sz, c_float, vp,
+                             sz, sz, vp, sz, sz],
+            "gemmActivationGradient": [c_int, c_int, sz, sz, sz, c_float, vp, sz, sz, vp, sz, sz, c_int, vp, sz, sz, vp, sz, sz,
+                                       vp, sz],
+            "activationGradient": [sz, sz, vp, sz, sz, c_int, vp, sz, sz, vp, sz, sz, vp, sz] + groups,
+            "gemmGrouped": [c_int, sz, sz, sz, c_float, vp, sz, sz, vp, sz, sz, sz, vp, sz, sz, c_int, vp, sz, sz, c_float, vp,
+                            sz, sz] + groups,
+            "gemmGroupedGradient": [sz, sz, sz, c_float, vp, sz, sz, vp, sz, sz, c_float, vp, sz, sz, sz] + groups,
+        }
+        for routine in LAYER_ROUTINES:
+            f = getattr(lib, "CLBlast%s%s" % (prefix, routine))
+            f.argtypes, f.restype = layer[routine] + [vp, vp], c_int
     for prefix in "SDH":
         f = getattr(lib, "CLBlast%sconvgemm" % prefix)
         f.argtypes = [c_int] + [sz] * 13 + [vp, sz, vp, sz, vp, sz, vp, vp]
@@ -128,7 +146,7 @@ C_API_SYMBOLS = (
     ["CLBlast%sgemm%s" % (p, s) for p in "CZ" for s in ("Batched", "StridedBatched")] +
     ["CLBlast%s%s" % (p, r) for p in "CZ" for r in ("symm", "hemm", "syrk", "herk", "syr2k", "her2k", "trmm", "trsm")] +
     ["CLBlast%s%s" % (p, r) for p in "SDH" for r in ("symm", "syrk", "syr2k", "trmm")] + ["CLBlastStrsm", "CLBlastDtrsm"] +
-    ["CLBlast%sconvgemm" % p for p in "SDH"] +
+    ["CLBlast%sconvgemm" % p for p in "SDH"] + ["CLBlast%s%s" % (p, r) for p in "SHB" for r in LAYER_ROUTINES] +
     ["CLBlastSgemmNoAlloc", "CLBlastClearCache", "CLBlastOverrideParameters", "CLBlastFloatToHalf", "CLBlastHalfToFloat"])
 NETLIB_SYMBOLS = (["cblas_%sgemm" % p for p in "sdcz"] +
                   ["cblas_%s%s" % (p, r) for p in "sdcz" for r in ("symm", "syrk", "syr2k", "trmm", "trsm")] +
@@ -138,7 +156,7 @@ DEVICE_LAYER_SYMBOLS = [
     "clbh_upload_async", "clbh_event_record", "clbh_stream_device", "clbh_error_string", "clbh_symmetric_to_square",
     "clbh_triangular_to_square", "clbh_triangular_to_band", "clbh_complex_triangular_to_band", "clbh_copy_matrix", "clbh_invert_block_size", "clbh_invert_diagonal_blocks",
     "clbh_complex_expand", "clbh_complex_transpose", "clbh_complex_scale", "clbh_complex_expand_batched",
-    "clbh_complex_transpose_batched", "clbh_complex_scale_batched", "clbh_complex_gemm_small_batched", "clbh_copy_matrix_batched", "clbh_alloc", "clbh_free", "clbh_copy", "clbh_im2col", "clbh_conv_gather_possible", "clbh_conv_slab_scratch_bytes", "clbh_conv_slab", "clbh_pad_image", "clbh_fill_zero", "clbh_complex_symmetric_to_square",
+    "clbh_complex_transpose_batched", "clbh_complex_scale_batched", "clbh_complex_gemm_small_batched", "clbh_copy_matrix_batched", "clbh_alloc", "clbh_free", "clbh_copy", "clbh_im2col", "clbh_conv_gather_possible", "clbh_conv_slab_scratch_bytes", "clbh_conv_slab", "clbh_layer_operands_fit", "clbh_layer_workspace_bytes", "clbh_layer_launch", "clbh_pad_image", "clbh_fill_zero", "clbh_complex_symmetric_to_square",
     "clbh_complex_triangular_to_square", "clbh_complex_zero_diagonal_imag", "clbh_complex_invert_block_size",
     "clbh_complex_invert_diagonal_blocks", "clbh_static_scratch", "clbh_static_scratch_bytes", "clbh_stream_capturing",
     "clbh_stream_is_alias", "clbh_compute_units", "clbh_tickets"]

@@ -21,10 +21,13 @@ TRIANGLE_UPPER, TRIANGLE_LOWER = 121, 122
 SIDE_LEFT, SIDE_RIGHT = 141, 142
 DIAGONAL_NON_UNIT, DIAGONAL_UNIT = 131, 132
 CROSS_CORRELATION, CONVOLUTION = 151, 152
+ACTIVATIONS = {"none": 161, "relu": 162, "gelu": 163, "gelu_tanh": 164, "silu": 165}
 
 STATUS_NAMES = {
     0: "kSuccess", -4: "kTempBufferAllocFailure", -30: "kInvalidValue", -36: "kInvalidCommandQueue",
     -1024: "kNotImplemented", -1022: "kInvalidMatrixA", -1021: "kInvalidMatrixB", -1020: "kInvalidMatrixC",
+    -1019: "kInvalidVectorX", -1018: "kInvalidVectorY", -1013: "kInvalidIncrementX", -1008: "kInsufficientMemoryX",
+    -1007: "kInsufficientMemoryY",
     -1017: "kInvalidDimension", -1016: "kInvalidLeadDimA", -1015: "kInvalidLeadDimB", -1014: "kInvalidLeadDimC",
     -1011: "kInsufficientMemoryA", -1010: "kInsufficientMemoryB", -1009: "kInsufficientMemoryC",
     -2050: "kInsufficientMemoryTemp", -2049: "kInvalidBatchCount", -2048: "kInvalidOverrideKernel",
@@ -389,3 +392,94 @@ def gemmStridedBatched(queue, m, n, k, batch_count, a, b, c, a_ld, b_ld, c_ld, a
                                       c_offset, c_ld, c_stride, batch_count, _stream_handle(queue))
     if status != 0:
         raise CLBlastError("CLBlast%sgemmStridedBatched" % prefix, status)
+
+
+# ---- products of a network's layers --------------------------------------------------------------------
+# Row-major, like the calls above, for float32, float16 and bfloat16 tensors; ``queue`` None is the current stream. Optional
+# tensors are None. ``activation`` is one of ACTIVATIONS. The headers describe the operators (include/clblast_hip.h).
+
+_LAYER_PREFIX = {"torch.float32": "S", "torch.float16": "H", "torch.bfloat16": "B"}
+
+
+def _layer(routine, queue, tensors, group_offsets, arguments):
+    first = tensors[0]
+    for t in tensors:
+        if t is not None:
+            if t.dtype != first.dtype:
+                raise ValueError("PyCLBlast: All arrays have to be of the same data-type, got: %s and %s" % (first.dtype, t.dtype))
+            if not t.is_cuda or t.device != first.device:
+                raise ValueError("PyCLBlast: operands must live on one GPU")
+    if group_offsets is not None:
+        if str(group_offsets.dtype) != "torch.int64" or not group_offsets.is_contiguous():
+            raise ValueError("PyCLBlast: group_offsets must be contiguous 64-bit integers")
+        if group_offsets.device != first.device:
+            raise ValueError("PyCLBlast: operands must live on one GPU")
+    prefix = _LAYER_PREFIX.get(str(first.dtype))
+    if prefix is None:
+        raise ValueError("PyCLBlast: unrecognized data-type '%s'" % first.dtype)
+    if queue is None:  # (the stream's device must be the current one, and so must the operands')
+        import torch
+        if first.device.index != torch.cuda.current_device():
+            raise ValueError("PyCLBlast: operands must live on the current GPU")
+    function = getattr(_lib.load(), "CLBlast%s%s" % (prefix, routine))
+    status = function(*arguments, _stream_ref(_stream_handle(queue)), None)
+    if status != 0:
+        raise CLBlastError("CLBlast%s%s" % (prefix, routine), status)
+
+
+def _activation(name):
+    try:
+        return ACTIVATIONS[name]
+    except KeyError:
+        raise ValueError("PyCLBlast: unknown activation '%s'" % name)
+
+
+def _ptr(tensor):
+    return None if tensor is None else tensor.data_ptr()
+
+
+def gemmEpilogue(queue, m, n, k, a, b, c, a_ld, b_ld, c_ld, alpha=1.0, beta=0.0, a_transp=False, b_transp=False, bias=None,
+                 activation="none", pre=None, pre_ld=0, residual=None, residual_ld=0, a_offset=0, b_offset=0, c_offset=0,
+                 bias_offset=0, pre_offset=0, residual_offset=0):
+    """c = act(alpha op(a) op(b) + bias) + beta residual; the activation's input is kept in `pre` unless that is None."""
+    _layer("gemmEpilogue", queue, (a, b, c, bias, pre, residual), None, (
+        TRANS_YES if a_transp else TRANS_NO, TRANS_YES if b_transp else TRANS_NO, m, n, k, alpha, a.data_ptr(), a_offset, a_ld,
+        b.data_ptr(), b_offset, b_ld, _ptr(bias), bias_offset, _activation(activation), _ptr(pre), pre_offset, pre_ld, beta,
+        _ptr(residual), residual_offset, residual_ld, c.data_ptr(), c_offset, c_ld))
+
+
+def gemmActivationGradient(queue, m, n, k, a, b, pre, c, a_ld, b_ld, pre_ld, c_ld, alpha=1.0, a_transp=False, b_transp=False,
+                           activation="none", bias_gradient=None, a_offset=0, b_offset=0, pre_offset=0, c_offset=0,
+                           bias_gradient_offset=0):
+    """c = (alpha op(a) op(b)) * act'(pre), bias_gradient = the column sums of c unless it is None."""
+    _layer("gemmActivationGradient", queue, (a, b, c, pre, bias_gradient), None, (
+        TRANS_YES if a_transp else TRANS_NO, TRANS_YES if b_transp else TRANS_NO, m, n, k, alpha, a.data_ptr(), a_offset, a_ld,
+        b.data_ptr(), b_offset, b_ld, _activation(activation), _ptr(pre), pre_offset, pre_ld, c.data_ptr(), c_offset, c_ld,
+        _ptr(bias_gradient), bias_gradient_offset))
+
+
+def activationGradient(queue, m, n, y, pre, c, y_ld, pre_ld, c_ld, activation="none", bias_gradient=None, group_count=1,
+                       group_offsets=None, y_offset=0, pre_offset=0, c_offset=0, bias_gradient_offset=0, group_offsets_offset=0):
+    """c = y * act'(pre), bias_gradient = the column sums of c over each group's rows (over all rows without groups); either
+    of the two outputs may be None."""
+    _layer("activationGradient", queue, (y, pre, c, bias_gradient), group_offsets, (
+        m, n, y.data_ptr(), y_offset, y_ld, _activation(activation), _ptr(pre), pre_offset, pre_ld, _ptr(c), c_offset, c_ld,
+        _ptr(bias_gradient), bias_gradient_offset, group_count, _ptr(group_offsets), group_offsets_offset))
+
+
+def gemmGrouped(queue, group_count, m, n, k, a, b, c, group_offsets, a_ld, b_ld, c_ld, b_stride, alpha=1.0, beta=0.0,
+                b_transp=False, bias=None, bias_stride=None, activation="none", pre=None, pre_ld=0, a_offset=0, b_offset=0,
+                c_offset=0, bias_offset=0, pre_offset=0, group_offsets_offset=0):
+    """For the rows group_offsets[g] .. group_offsets[g + 1] - 1 of a, c and pre: c = act(alpha a op(b[g]) + bias[g]) + beta c."""
+    _layer("gemmGrouped", queue, (a, b, c, bias, pre), group_offsets, (
+        TRANS_YES if b_transp else TRANS_NO, m, n, k, alpha, a.data_ptr(), a_offset, a_ld, b.data_ptr(), b_offset, b_ld, b_stride,
+        _ptr(bias), bias_offset, n if bias_stride is None else bias_stride, _activation(activation), _ptr(pre), pre_offset, pre_ld,
+        beta, c.data_ptr(), c_offset, c_ld, group_count, group_offsets.data_ptr(), group_offsets_offset))
+
+
+def gemmGroupedGradient(queue, group_count, k, m, n, a, b, c, group_offsets, a_ld, b_ld, c_ld, c_stride, alpha=1.0, beta=0.0,
+                        a_offset=0, b_offset=0, c_offset=0, group_offsets_offset=0):
+    """c[g] = alpha a_g^T b_g + beta c[g], a_g and b_g being the rows group_offsets[g] .. group_offsets[g + 1] - 1 of a and b."""
+    _layer("gemmGroupedGradient", queue, (a, b, c), group_offsets, (
+        m, n, k, alpha, a.data_ptr(), a_offset, a_ld, b.data_ptr(), b_offset, b_ld, beta, c.data_ptr(), c_offset, c_ld, c_stride,
+        group_count, group_offsets.data_ptr(), group_offsets_offset))

@@ -16,6 +16,7 @@
 #include "routines/xgemmbatched_complex.hpp"
 #include "routines/xconvgemm.hpp"
 #include "routines/xgemmbatched.hpp"
+#include "routines/xlayer.hpp"
 #include "routines/xsymm.hpp"
 #include "routines/xsyrk.hpp"
 #include "routines/xtrmm.hpp"
@@ -276,6 +277,123 @@ CLBLAST_HIP_INSTANTIATE(half)
 CLBLAST_HIP_INSTANTIATE(float)
 CLBLAST_HIP_INSTANTIATE(double)
 #undef CLBLAST_HIP_INSTANTIATE
+
+// ---- products of a network's layers (routines/xlayer.cpp) ---------------------------------------------------------------
+template <typename T>
+StatusCode GemmEpilogue(const Transpose a_transpose, const Transpose b_transpose, const size_t m, const size_t n,
+                        const size_t k, const float alpha, const void* a_buffer, const size_t a_offset, const size_t a_ld,
+                        const void* b_buffer, const size_t b_offset, const size_t b_ld, const void* bias_buffer,
+                        const size_t bias_offset, const Activation activation, void* pre_buffer, const size_t pre_offset,
+                        const size_t pre_ld, const float beta, const void* residual_buffer,
+                        const size_t residual_offset, const size_t residual_ld, void* c_buffer, const size_t c_offset,
+                        const size_t c_ld, hipStream_t* queue, hipEvent_t* event) {
+  try {
+    auto routine = Xlayer<T>(queue, event);
+    routine.DoGemmEpilogue(a_transpose, b_transpose, m, n, k, alpha, {a_buffer, a_offset, a_ld}, {b_buffer, b_offset,
+                           b_ld}, {bias_buffer, bias_offset, 0}, activation, {pre_buffer, pre_offset, pre_ld}, beta,
+                           {residual_buffer, residual_offset, residual_ld}, {c_buffer, c_offset, c_ld});
+    return StatusCode::kSuccess;
+  } catch (...) {
+    return DispatchException();
+  }
+}
+
+template <typename T>
+StatusCode GemmActivationGradient(const Transpose a_transpose, const Transpose b_transpose, const size_t m,
+                                  const size_t n, const size_t k, const float alpha, const void* a_buffer, const size_t a_offset,
+                                  const size_t a_ld, const void* b_buffer, const size_t b_offset, const size_t b_ld,
+                                  const Activation activation, const void* pre_buffer, const size_t pre_offset,
+                                  const size_t pre_ld, void* c_buffer, const size_t c_offset, const size_t c_ld,
+                                  void* bias_gradient_buffer, const size_t bias_gradient_offset, hipStream_t* queue,
+                                  hipEvent_t* event) {
+  try {
+    auto routine = Xlayer<T>(queue, event);
+    routine.DoGemmActivationGradient(a_transpose, b_transpose, m, n, k, alpha, {a_buffer, a_offset, a_ld}, {b_buffer,
+                                     b_offset, b_ld}, activation, {pre_buffer, pre_offset, pre_ld}, {c_buffer, c_offset,
+                                     c_ld}, {bias_gradient_buffer, bias_gradient_offset, 0});
+    return StatusCode::kSuccess;
+  } catch (...) {
+    return DispatchException();
+  }
+}
+
+template <typename T>
+StatusCode ActivationGradient(const size_t m, const size_t n, const void* y_buffer, const size_t y_offset,
+                              const size_t y_ld, const Activation activation, const void* pre_buffer, const size_t pre_offset,
+                              const size_t pre_ld, void* c_buffer, const size_t c_offset, const size_t c_ld,
+                              void* bias_gradient_buffer, const size_t bias_gradient_offset, const size_t group_count,
+                              const void* group_offsets, const size_t group_offsets_offset, hipStream_t* queue,
+                              hipEvent_t* event) {
+  try {
+    auto routine = Xlayer<T>(queue, event);
+    routine.DoActivationGradient(m, n, {y_buffer, y_offset, y_ld}, activation, {pre_buffer, pre_offset, pre_ld},
+                                 {c_buffer, c_offset, c_ld}, {bias_gradient_buffer, bias_gradient_offset, n},
+                                 {group_count, group_offsets, group_offsets_offset});
+    return StatusCode::kSuccess;
+  } catch (...) {
+    return DispatchException();
+  }
+}
+
+template <typename T>
+StatusCode GemmGrouped(const Transpose b_transpose, const size_t m, const size_t n, const size_t k, const float alpha,
+                       const void* a_buffer, const size_t a_offset, const size_t a_ld, const void* b_buffer,
+                       const size_t b_offset, const size_t b_ld, const size_t b_stride, const void* bias_buffer,
+                       const size_t bias_offset, const size_t bias_stride, const Activation activation, void* pre_buffer,
+                       const size_t pre_offset, const size_t pre_ld, const float beta, void* c_buffer, const size_t c_offset,
+                       const size_t c_ld, const size_t group_count, const void* group_offsets,
+                       const size_t group_offsets_offset, hipStream_t* queue, hipEvent_t* event) {
+  try {
+    auto routine = Xlayer<T>(queue, event);
+    routine.DoGemmGrouped(b_transpose, m, n, k, alpha, {a_buffer, a_offset, a_ld}, {b_buffer, b_offset, b_ld}, b_stride,
+                          {bias_buffer, bias_offset, bias_stride}, activation, {pre_buffer, pre_offset, pre_ld}, beta,
+                          {c_buffer, c_offset, c_ld}, {group_count, group_offsets, group_offsets_offset});
+    return StatusCode::kSuccess;
+  } catch (...) {
+    return DispatchException();
+  }
+}
+
+template <typename T>
+StatusCode GemmGroupedGradient(const size_t m, const size_t n, const size_t k, const float alpha, const void* a_buffer,
+                               const size_t a_offset, const size_t a_ld, const void* b_buffer, const size_t b_offset,
+                               const size_t b_ld, const float beta, void* c_buffer, const size_t c_offset,
+                               const size_t c_ld, const size_t c_stride, const size_t group_count, const void* group_offsets,
+                               const size_t group_offsets_offset, hipStream_t* queue, hipEvent_t* event) {
+  try {
+    auto routine = Xlayer<T>(queue, event);
+    routine.DoGemmGroupedGradient(m, n, k, alpha, {a_buffer, a_offset, a_ld}, {b_buffer, b_offset, b_ld}, beta,
+                                  {c_buffer, c_offset, c_ld}, c_stride, {group_count, group_offsets,
+                                  group_offsets_offset});
+    return StatusCode::kSuccess;
+  } catch (...) {
+    return DispatchException();
+  }
+}
+
+#define CLBLAST_HIP_INSTANTIATE_LAYER(T) \
+    template StatusCode CLBLAST_HIP_PUBLIC GemmEpilogue<T>(const Transpose, const Transpose, const size_t, \
+      const size_t, const size_t, const float, const void*, const size_t, const size_t, const void*, const size_t, \
+      const size_t, const void*, const size_t, const Activation, void*, const size_t, const size_t, const float, \
+      const void*, const size_t, const size_t, void*, const size_t, const size_t, hipStream_t*, hipEvent_t*); \
+    template StatusCode CLBLAST_HIP_PUBLIC GemmActivationGradient<T>(const Transpose, const Transpose, const size_t, \
+      const size_t, const size_t, const float, const void*, const size_t, const size_t, const void*, const size_t, \
+      const size_t, const Activation, const void*, const size_t, const size_t, void*, const size_t, const size_t, \
+      void*, const size_t, hipStream_t*, hipEvent_t*); \
+    template StatusCode CLBLAST_HIP_PUBLIC ActivationGradient<T>(const size_t, const size_t, const void*, \
+      const size_t, const size_t, const Activation, const void*, const size_t, const size_t, void*, const size_t, \
+      const size_t, void*, const size_t, const size_t, const void*, const size_t, hipStream_t*, hipEvent_t*); \
+    template StatusCode CLBLAST_HIP_PUBLIC GemmGrouped<T>(const Transpose, const size_t, const size_t, const size_t, \
+      const float, const void*, const size_t, const size_t, const void*, const size_t, const size_t, const size_t, \
+      const void*, const size_t, const size_t, const Activation, void*, const size_t, const size_t, const float, \
+      void*, const size_t, const size_t, const size_t, const void*, const size_t, hipStream_t*, hipEvent_t*); \
+    template StatusCode CLBLAST_HIP_PUBLIC GemmGroupedGradient<T>(const size_t, const size_t, const size_t, \
+      const float, const void*, const size_t, const size_t, const void*, const size_t, const size_t, const float, void*, \
+      const size_t, const size_t, const size_t, const size_t, const void*, const size_t, hipStream_t*, hipEvent_t*);
+CLBLAST_HIP_INSTANTIATE_LAYER(half)
+CLBLAST_HIP_INSTANTIATE_LAYER(float)
+CLBLAST_HIP_INSTANTIATE_LAYER(bfloat16)
+#undef CLBLAST_HIP_INSTANTIATE_LAYER
 
 // CGEMM and ZGEMM (reference: src/clblast.cpp:1093-1100)
 template <typename R>

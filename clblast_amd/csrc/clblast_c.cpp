@@ -15,6 +15,7 @@
 namespace {
 inline clblast::Layout L(const CLBlastLayout v) { return static_cast<clblast::Layout>(v); }
 inline clblast::Transpose Tr(const CLBlastTranspose v) { return static_cast<clblast::Transpose>(v); }
+inline clblast::Activation Ac(const CLBlastActivation v) { return static_cast<clblast::Activation>(v); }
 template <typename F>
 CLBlastStatusCode Guarded(F&& body) {
   try {
@@ -328,6 +329,99 @@ CLBlastStatusCode CLBlastHsymm(const CLBlastLayout layout, const CLBlastSide sid
 CLBLAST_HIP_CONVGEMM(CLBlastSconvgemm, float)
 CLBLAST_HIP_CONVGEMM(CLBlastDconvgemm, double)
 CLBLAST_HIP_CONVGEMM(CLBlastHconvgemm, clblast::half)
+
+// ---- products of a network's layers --------------------------------------------------------------
+#define CLBLAST_HIP_GEMMEPILOGUE(NAME, T) \
+  CLBlastStatusCode NAME(const CLBlastTranspose a_transpose, const CLBlastTranspose b_transpose, const size_t m, \
+      const size_t n, const size_t k, const float alpha, const void* a_buffer, const size_t a_offset, \
+      const size_t a_ld, const void* b_buffer, const size_t b_offset, const size_t b_ld, const void* bias_buffer, \
+      const size_t bias_offset, const CLBlastActivation activation, void* pre_buffer, const size_t pre_offset, \
+      const size_t pre_ld, const float beta, const void* residual_buffer, const size_t residual_offset, \
+      const size_t residual_ld, void* c_buffer, const size_t c_offset, const size_t c_ld, hipStream_t* queue, \
+      hipEvent_t* event) { \
+    return Guarded([&]() { \
+      return clblast::GemmEpilogue<T>(Tr(a_transpose), Tr(b_transpose), m, n, k, alpha, a_buffer, a_offset, \
+          a_ld, b_buffer, b_offset, b_ld, bias_buffer, bias_offset, Ac(activation), pre_buffer, pre_offset, \
+          pre_ld, beta, residual_buffer, residual_offset, residual_ld, c_buffer, c_offset, c_ld, queue, \
+          event); \
+    }); \
+  }
+CLBLAST_HIP_GEMMEPILOGUE(CLBlastSgemmEpilogue, float)
+CLBLAST_HIP_GEMMEPILOGUE(CLBlastHgemmEpilogue, clblast::half)
+CLBLAST_HIP_GEMMEPILOGUE(CLBlastBgemmEpilogue, clblast::bfloat16)
+#undef CLBLAST_HIP_GEMMEPILOGUE
+
+#define CLBLAST_HIP_GEMMACTIVATIONGRADIENT(NAME, T) \
+  CLBlastStatusCode NAME(const CLBlastTranspose a_transpose, const CLBlastTranspose b_transpose, const size_t m, \
+      const size_t n, const size_t k, const float alpha, const void* a_buffer, const size_t a_offset, \
+      const size_t a_ld, const void* b_buffer, const size_t b_offset, const size_t b_ld, \
+      const CLBlastActivation activation, const void* pre_buffer, const size_t pre_offset, const size_t pre_ld, void* c_buffer, \
+      const size_t c_offset, const size_t c_ld, void* bias_gradient_buffer, const size_t bias_gradient_offset, \
+      hipStream_t* queue, hipEvent_t* event) { \
+    return Guarded([&]() { \
+      return clblast::GemmActivationGradient<T>(Tr(a_transpose), Tr(b_transpose), m, n, k, alpha, a_buffer, \
+          a_offset, a_ld, b_buffer, b_offset, b_ld, Ac(activation), pre_buffer, pre_offset, pre_ld, c_buffer, \
+          c_offset, c_ld, bias_gradient_buffer, bias_gradient_offset, queue, event); \
+    }); \
+  }
+CLBLAST_HIP_GEMMACTIVATIONGRADIENT(CLBlastSgemmActivationGradient, float)
+CLBLAST_HIP_GEMMACTIVATIONGRADIENT(CLBlastHgemmActivationGradient, clblast::half)
+CLBLAST_HIP_GEMMACTIVATIONGRADIENT(CLBlastBgemmActivationGradient, clblast::bfloat16)
+#undef CLBLAST_HIP_GEMMACTIVATIONGRADIENT
+
+#define CLBLAST_HIP_ACTIVATIONGRADIENT(NAME, T) \
+  CLBlastStatusCode NAME(const size_t m, const size_t n, const void* y_buffer, const size_t y_offset, \
+      const size_t y_ld, const CLBlastActivation activation, const void* pre_buffer, const size_t pre_offset, \
+      const size_t pre_ld, void* c_buffer, const size_t c_offset, const size_t c_ld, void* bias_gradient_buffer, \
+      const size_t bias_gradient_offset, const size_t group_count, const void* group_offsets, \
+      const size_t group_offsets_offset, hipStream_t* queue, hipEvent_t* event) { \
+    return Guarded([&]() { \
+      return clblast::ActivationGradient<T>(m, n, y_buffer, y_offset, y_ld, Ac(activation), pre_buffer, \
+          pre_offset, pre_ld, c_buffer, c_offset, c_ld, bias_gradient_buffer, bias_gradient_offset, \
+          group_count, group_offsets, group_offsets_offset, queue, event); \
+    }); \
+  }
+CLBLAST_HIP_ACTIVATIONGRADIENT(CLBlastSactivationGradient, float)
+CLBLAST_HIP_ACTIVATIONGRADIENT(CLBlastHactivationGradient, clblast::half)
+CLBLAST_HIP_ACTIVATIONGRADIENT(CLBlastBactivationGradient, clblast::bfloat16)
+#undef CLBLAST_HIP_ACTIVATIONGRADIENT
+
+#define CLBLAST_HIP_GEMMGROUPED(NAME, T) \
+  CLBlastStatusCode NAME(const CLBlastTranspose b_transpose, const size_t m, const size_t n, const size_t k, \
+      const float alpha, const void* a_buffer, const size_t a_offset, const size_t a_ld, const void* b_buffer, \
+      const size_t b_offset, const size_t b_ld, const size_t b_stride, const void* bias_buffer, \
+      const size_t bias_offset, const size_t bias_stride, const CLBlastActivation activation, void* pre_buffer, \
+      const size_t pre_offset, const size_t pre_ld, const float beta, void* c_buffer, const size_t c_offset, \
+      const size_t c_ld, const size_t group_count, const void* group_offsets, const size_t group_offsets_offset, \
+      hipStream_t* queue, hipEvent_t* event) { \
+    return Guarded([&]() { \
+      return clblast::GemmGrouped<T>(Tr(b_transpose), m, n, k, alpha, a_buffer, a_offset, a_ld, b_buffer, \
+          b_offset, b_ld, b_stride, bias_buffer, bias_offset, bias_stride, Ac(activation), pre_buffer, \
+          pre_offset, pre_ld, beta, c_buffer, c_offset, c_ld, group_count, group_offsets, \
+          group_offsets_offset, queue, event); \
+    }); \
+  }
+CLBLAST_HIP_GEMMGROUPED(CLBlastSgemmGrouped, float)
+CLBLAST_HIP_GEMMGROUPED(CLBlastHgemmGrouped, clblast::half)
+CLBLAST_HIP_GEMMGROUPED(CLBlastBgemmGrouped, clblast::bfloat16)
+#undef CLBLAST_HIP_GEMMGROUPED
+
+#define CLBLAST_HIP_GEMMGROUPEDGRADIENT(NAME, T) \
+  CLBlastStatusCode NAME(const size_t m, const size_t n, const size_t k, const float alpha, \
+      const void* a_buffer, const size_t a_offset, const size_t a_ld, const void* b_buffer, const size_t b_offset, \
+      const size_t b_ld, const float beta, void* c_buffer, const size_t c_offset, const size_t c_ld, \
+      const size_t c_stride, const size_t group_count, const void* group_offsets, const size_t group_offsets_offset, \
+      hipStream_t* queue, hipEvent_t* event) { \
+    return Guarded([&]() { \
+      return clblast::GemmGroupedGradient<T>(m, n, k, alpha, a_buffer, a_offset, a_ld, b_buffer, b_offset, \
+          b_ld, beta, c_buffer, c_offset, c_ld, c_stride, group_count, group_offsets, group_offsets_offset, \
+          queue, event); \
+    }); \
+  }
+CLBLAST_HIP_GEMMGROUPEDGRADIENT(CLBlastSgemmGroupedGradient, float)
+CLBLAST_HIP_GEMMGROUPEDGRADIENT(CLBlastHgemmGroupedGradient, clblast::half)
+CLBLAST_HIP_GEMMGROUPEDGRADIENT(CLBlastBgemmGroupedGradient, clblast::bfloat16)
+#undef CLBLAST_HIP_GEMMGROUPEDGRADIENT
 
 // ---- CGEMM, ZGEMM -------------------------------------------------------------------------------
 CLBlastStatusCode CLBlastCgemm(const CLBlastLayout layout, const CLBlastTranspose a_transpose,

@@ -609,7 +609,7 @@ __global__ __launch_bounds__(Config::THREADS, Config::MIN_WAVES) void HgemmDirec
 
 // Second pass of a split-K launch: C = alpha * (sum of the fp32 workspace slabs) + beta * C, rounded to fp16 once.
 // grid: (ceil(m / 256), n).
-__global__ __launch_bounds__(256) void HgemmSplitReduceKernel(const float* __restrict__ workspace, const int splits,
+static __global__ __launch_bounds__(256) void HgemmSplitReduceKernel(const float* __restrict__ workspace, const int splits,
                                                               const int split_ld, _Float16* __restrict__ c,
                                                               const long long c_ld, const int m, const int n,
                                                               const float alpha, const float beta) {

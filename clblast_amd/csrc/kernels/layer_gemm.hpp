@@ -1,0 +1,775 @@
+// =================================================================================================
+// Products of a network's layers for gfx950: fp32, fp16 and bf16, sums in fp32, with the layer's elementwise work in the
+// epilogue and, where the rows belong to groups (experts), every group multiplied by its own matrix in the same launch.
+//
+// Canonical problem (the caller's row-major matrices read as column-major ones): C(i, j) for i < m features - contiguous in
+// C - and j < n rows,
+//   S(i, j) = sum_p A(i, p) B(p, j)         A: the weights, B: the rows the layer is applied to
+//   forward:   Z = alpha S + bias(i)        C = act(Z) + beta R(i, j)        (Z stored too where `pre` is set)
+//   gradient:  C = alpha S act'(Z(i, j))    Z read from `pre`; sums of C over the tile's rows go to `bias_partials`
+// Groups by rows:  group g owns the rows offsets[g] .. offsets[g + 1] - 1 of B, C and pre, and has its own A and bias.
+// Groups by depth: group g owns that range of p in A and B, and has its own C: the gradients of the groups' weights.
+// The offsets lie in device memory; they are clamped to the rows that exist, so no offset leads outside a matrix.
+//
+// Structure: a work-group owns a TILE_M x TILE_N tile, K is walked in slabs of 64 bytes per line (32 halfs, 16 floats) in a
+// ring of three LDS buffers. Both types share the byte layout of a slab, the direct global -> LDS requests (16 bytes per lane, range-checked
+// by the buffer resource), the one barrier per slab and the order of products: the wavefront's blocks form four quadrants
+// whose missing fragments are read under the products of the quadrant before. What differs is the instruction: 16 bits
+// v_mfma_f32_16x16x32_{f16,bf16}, a slab is one instruction deep, and x-contiguous operands are read with the transposing LDS
+// read; fp32 v_mfma_f32_32x32x2_f32 (16x16x4 on the smallest tile), where lane half h feeds the depths 4h + s and
+// 8 + 4h + s (s = 0..3) in both operands, so that a k-contiguous operand is read in 16-byte pieces and an
+// x-contiguous one value by value, neither of them transposed.
+//
+// Epilogue: half of its rows at a time, a wavefront writes its sums to LDS in fp32 as [row][feature] and reads them back with
+// consecutive lanes along the features, so that bias, residual, Z and C all move in 16-byte pieces of whole lines, and a
+// lane keeps the same features for the whole tile (its bias values and its part of the bias gradient stay in registers).
+// Only the final value is rounded.
+// =================================================================================================
+#ifndef CLBLAST_HIP_KERNELS_LAYER_GEMM_HPP_
+#define CLBLAST_HIP_KERNELS_LAYER_GEMM_HPP_
+
+#include <type_traits>
+
+#include "kernels/activations.hpp"
+#include "kernels/gemm_direct_f16.hpp"
+#include "kernels/gemm_mfma.hpp"
+
+namespace clbh {
+
+constexpr int kLayerPlain = 0, kLayerGroupedRows = 1, kLayerGroupedDepth = 2;
+
+struct LayerArgs {
+  const void* a;
+  const void* b;
+  void* c;
+  long long a_ld, b_ld, c_ld;
+  long long a_stride, c_stride;  // from one group's A (groups by rows) or C (groups by depth) to the next one's
+  int m, n, k;                   // n: all rows there are; k: the depth, for groups by depth all of it
+  float alpha, beta;
+  const void* bias;  // or nullptr
+  long long bias_stride;
+  void* pre;  // Z: written (forward, or nullptr), read (gradient)
+  long long pre_ld;
+  const void* residual;  // not read when beta == 0
+  long long residual_ld;
+  int activation;
+  int gradient;
+  int grouping;  // kLayerPlain, ...
+  int groups;
+  const long long* offsets;  // groups + 1 values
+  int vector_rows;           // C, pre, residual and bias can be moved in 16-byte pieces (dword-aligned rows)
+  float* bias_partials;      // [tile of rows][m], or nullptr
+  // K ranges of one plain product: range s goes to partials + s * n * m as fp32 sums, a second kernel finishes
+  int split_chunk;
+  float* partials;
+};
+
+// ---- group lookup ------------------------------------------------------------------------------------------------------
+
+// The rows of group g, inside 0 .. rows whatever the offsets say
+__device__ __forceinline__ void GroupRange(const long long* offsets, const int g, const int rows, int& begin, int& end) {
+  const long long first = UniformRead(offsets + g), last = UniformRead(offsets + g + 1);
+  begin = static_cast<int>(first < 0 ? 0 : (first > rows ? rows : first));
+  end = static_cast<int>(last < begin ? begin : (last > rows ? rows : last));
+}
+
+// No group of a valid call has more tiles than this: grouped calls have less than 2^26 rows, a tile has at least 8. Offsets
+// that are out of order can make the groups overlap; the numbers of tiles still fit 32 bits then.
+constexpr int kLayerMostGroupTiles = 1 << 23;
+
+// Every group's rows are cut into tiles of `tile` rows, numbered through from group 0 on. Sums up all tiles and finds the
+// group that owns tile `wanted` (a function of that sum): 64 groups at a time, one per lane, and a scan over the lanes.
+// wanted_of(total) returns the tile's number, or a negative one where this work-group has none. Uniform results;
+// returns false without a tile. `before`: tiles of the groups in front of the one found.
+template <typename Wanted>
+__device__ __forceinline__ bool FindGroupTile(const long long* __restrict__ offsets, const int groups, const int rows,
+                                              const int tile, const int lane, Wanted wanted_of, int& group, int& before,
+                                              int& begin, int& end) {
+  // `first`: the lane's first row, `count`: rows, `tiles`: up to and including the lane's group
+  int first = 0, count = 0, tiles = 0;
+  const auto load = [&](const int base) {
+    const int g = base + lane;
+    first = 0;
+    count = 0;
+    if (g < groups) {
+      const long long from = offsets[g], to = offsets[g + 1];
+      first = static_cast<int>(from < 0 ? 0 : (from > rows ? rows : from));
+      count = static_cast<int>(to < first ? 0 : (to > rows ? rows : to) - first);
+    }
+    tiles = min((count + tile - 1) / tile, kLayerMostGroupTiles);
+#pragma unroll
+    for (int step = 1; step < 64; step *= 2) {
+      const int other = __shfl_up(tiles, step, 64);
+      if (lane >= step) { tiles += other; }
+    }
+  };
+  int total = 0;
+  for (int base = 0; base < groups; base += 64) {
+    load(base);
+    total = min(total + __builtin_amdgcn_readlane(tiles, 63), 128 * kLayerMostGroupTiles);
+  }
+  const int wanted = wanted_of(total);
+  if (wanted < 0 || wanted >= total) { return false; }
+  int passed = 0;
+  for (int base = 0; base < groups; base += 64) {
+    if (groups > 64) { load(base); }
+    const int here = __builtin_amdgcn_readlane(tiles, 63);
+    if (wanted < passed + here) {
+      const unsigned long long reached = __ballot(passed + tiles > wanted);
+      const int owner = __builtin_ctzll(reached);
+      group = base + owner;
+      begin = __builtin_amdgcn_readlane(first, owner);
+      end = begin + __builtin_amdgcn_readlane(count, owner);
+      before = passed + ((owner > 0) ? __builtin_amdgcn_readlane(tiles, (owner > 0) ? owner - 1 : 0) : 0);
+      return true;
+    }
+    passed += here;
+  }
+  return false;
+}
+
+// ---- types and configurations ------------------------------------------------------------------------------------------
+
+typedef short short8_t __attribute__((ext_vector_type(8)));
+typedef __bf16 bfloat8_t __attribute__((ext_vector_type(8)));
+typedef float layer_float4_t __attribute__((ext_vector_type(4)));
+typedef float layer_float8_t __attribute__((ext_vector_type(8)));
+
+// WM x WN wavefronts, each owning (32 FM) x (32 FN) of the tile; BLOCK: extent of the matrix instruction's block.
+template <typename T_, int WM_, int WN_, int FM_, int FN_, int MIN_WAVES_>
+struct LayerConfig {
+  using T = T_;
+  static constexpr int WM = WM_, WN = WN_, FM = FM_, FN = FN_, MIN_WAVES = MIN_WAVES_;
+  static constexpr int WAVES = WM * WN, THREADS = 64 * WAVES;
+  static constexpr int TILE_M = WM * FM * 32, TILE_N = WN * FN * 32;
+  static constexpr int TILE_K = 64 / sizeof(T);
+  static constexpr int VEC = 16 / sizeof(T);
+  static constexpr int BLOCK = (sizeof(T) == 4 && FM % 2 == 0 && FN % 2 == 0) ? 32 : 16;
+  static constexpr int BM = 32 * FM / BLOCK, BN = 32 * FN / BLOCK;  // the wavefront's blocks
+  static constexpr int STAGES = 3;
+  static constexpr int PIECES_A = TILE_M / 16, PIECES_B = TILE_N / 16;  // 1 KiB pieces of a slab
+  static constexpr int ROUNDS = (PIECES_A + PIECES_B + WAVES - 1) / WAVES;
+  static constexpr bool DUMMY = (PIECES_A + PIECES_B) % WAVES != 0;
+  static constexpr int A_BYTES = PIECES_A * 1024, B_BYTES = PIECES_B * 1024;
+  static constexpr int RING_BYTES = STAGES * (A_BYTES + B_BYTES) + (DUMMY ? 1024 : 0);
+  static constexpr int WAVE_M = 32 * FM, WAVE_N = 32 * FN;
+  static constexpr int PITCH = WAVE_M + 4;  // floats of a row of the epilogue's staging tile
+  static constexpr int HALF_N = WAVE_N / 2;  // rows that a wavefront stages at a time
+  static constexpr int STAGE_BYTES = HALF_N * PITCH * 4;
+  static constexpr int EPILOGUE_BYTES = WAVES * STAGE_BYTES;
+  static constexpr int SUM_BYTES = WN * TILE_M * 4;  // the wavefronts' parts of the bias gradient
+  static constexpr int LDS_BYTES = (RING_BYTES > EPILOGUE_BYTES + SUM_BYTES) ? RING_BYTES : EPILOGUE_BYTES + SUM_BYTES;
+  static_assert(BM % 2 == 0 && BN % 2 == 0 && BM >= BN, "the quadrants are halves of the blocks, walked along m");
+};
+
+template <typename Config> struct LayerMath;
+
+// Fragment reads and products of a slab, per type. Offsets are in bytes from the start of the operand's stage.
+template <typename Config>
+struct LayerMath16 {
+  using Frag = short8_t;
+  typedef float Acc __attribute__((ext_vector_type(4)));
+  template <int W, bool KC>
+  static __device__ __forceinline__ int Offset(const int lane, const int x0) { return 2 * HFragmentOffset<W, KC>(lane, x0); }
+  template <int W, bool KC>
+  static __device__ __forceinline__ Frag Read(const char* stage, const int offset) {
+    return __builtin_bit_cast(Frag, HFragment<W, KC>(reinterpret_cast<const _Float16*>(stage + offset), 0));
+  }
+  static __device__ __forceinline__ Acc Multiply(const Frag a, const Frag b, const Acc acc) {
+    if constexpr (std::is_same<typename Config::T, __bf16>::value) {
+      return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bfloat8_t, a), __builtin_bit_cast(bfloat8_t, b), acc, 0, 0, 0);
+    } else {
+      return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, a), __builtin_bit_cast(half8_t, b), acc, 0, 0, 0);
+    }
+  }
+};
+
+template <typename Config, int BLOCK> struct LayerMath32;
+template <typename Config>
+struct LayerMath32<Config, 32> {
+  using Frag = layer_float8_t;
+  using Acc = float16_t;
+  template <int W, bool KC>
+  static __device__ __forceinline__ int Offset(const int lane, const int x0) {
+    const int x = x0 + lane % 32, h = lane / 32;
+    return KC ? x * 64 : (4 * h * W + x) * 4;
+  }
+  template <int W, bool KC>
+  static __device__ __forceinline__ Frag Read(const char* stage, const int offset, const int lane) {
+    Frag out;
+    if constexpr (KC) {
+      // (offset is a multiple of 64 bytes: the row; its swizzle comes from the row's number)
+      const int h = lane / 32, swizzle = (offset >> 8) & 3;
+      const layer_float4_t low = *reinterpret_cast<const layer_float4_t*>(stage + offset + 16 * (h ^ swizzle));
+      const layer_float4_t high = *reinterpret_cast<const layer_float4_t*>(stage + offset + 16 * ((2 + h) ^ swizzle));
+#pragma unroll
+      for (int s = 0; s < 4; ++s) { out[s] = low[s]; out[4 + s] = high[s]; }
+    } else {
+      const float* from = reinterpret_cast<const float*>(stage + offset);
+#pragma unroll
+      for (int s = 0; s < 4; ++s) { out[s] = from[s * W]; out[4 + s] = from[(8 + s) * W]; }
+    }
+    return out;
+  }
+  static __device__ __forceinline__ Acc Multiply(const Frag a, const Frag b, Acc acc) {
+#pragma unroll
+    for (int s = 0; s < 8; ++s) { acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a[s], b[s], acc, 0, 0, 0); }
+    return acc;
+  }
+};
+template <typename Config>
+struct LayerMath32<Config, 16> {
+  using Frag = layer_float4_t;
+  typedef float Acc __attribute__((ext_vector_type(4)));
+  template <int W, bool KC>
+  static __device__ __forceinline__ int Offset(const int lane, const int x0) {
+    const int x = x0 + lane % 16, g = lane / 16;
+    return KC ? x * 64 + 16 * (g ^ ((x >> 2) & 3)) : (4 * g * W + x) * 4;
+  }
+  template <int W, bool KC>
+  static __device__ __forceinline__ Frag Read(const char* stage, const int offset, const int) {
+    if constexpr (KC) { return *reinterpret_cast<const Frag*>(stage + offset); }
+    Frag out;
+    const float* from = reinterpret_cast<const float*>(stage + offset);
+#pragma unroll
+    for (int s = 0; s < 4; ++s) { out[s] = from[s * W]; }
+    return out;
+  }
+  static __device__ __forceinline__ Acc Multiply(const Frag a, const Frag b, Acc acc) {
+#pragma unroll
+    for (int s = 0; s < 4; ++s) { acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a[s], b[s], acc, 0, 0, 0); }
+    return acc;
+  }
+};
+
+template <typename Config, bool WIDE = (sizeof(typename Config::T) == 4)> struct LayerMathOf { using type = LayerMath16<Config>; };
+template <typename Config> struct LayerMathOf<Config, true> { using type = LayerMath32<Config, Config::BLOCK>; };
+
+// ---- slab movement -----------------------------------------------------------------------------------------------------
+
+// Byte offset of a lane's 16 bytes from the first line of a 1 KiB piece. KC: 16 lines x of 64 bytes, the chunk swizzled
+// by (x >> 2) & 3; else lines k of W elements (16 bits: swizzled for the transposing read, fp32: in order).
+template <typename T, int W, bool KC>
+__device__ __forceinline__ int LayerPieceLaneBytes(const long long ld, const int piece, const int lane) {
+  constexpr int LINES = KC ? 16 : 1024 / (W * static_cast<int>(sizeof(T))), CHUNKS = 64 / LINES;
+  static_assert(LINES >= 1, "a piece holds whole lines");
+  const int line = lane / CHUNKS, position = lane % CHUNKS;
+  int chunk = position;
+  if constexpr (KC) { chunk = position ^ ((line >> 2) & 3); }
+  else if constexpr (sizeof(T) == 2) { chunk = position ^ HSwizzle<W>(LINES * piece + line); }
+  return static_cast<int>(line * ld * static_cast<long long>(sizeof(T))) + 16 * chunk;
+}
+
+template <bool RANGE, typename Tag>
+__device__ __forceinline__ void LayerRequestPiece(const char* source, const char* valid_end, char* destination, const int lane_bytes) {
+  typedef __attribute__((address_space(3))) void* LdsPtr;
+  const int records = RANGE ? HRecordsUpTo(source, valid_end) : -1;
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(__builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(source), 0, records, kRawBufferFlags),
+                                           (LdsPtr)(destination), 16, lane_bytes, 0, 0, 0);
+}
+
+// Zeroes the values k >= k_valid of a k-contiguous piece that this wavefront requested itself
+template <typename T>
+__device__ __forceinline__ void LayerZeroTail(char* stage, const int piece, const int lane, const int k_valid) {
+  constexpr int VEC = 16 / sizeof(T);
+  const int line = lane / 4, chunk = (lane % 4) ^ ((line >> 2) & 3);
+  T* cell = reinterpret_cast<T*>(stage + piece * 1024 + lane * 16);
+  if (VEC * chunk + VEC - 1 >= k_valid) {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) { if (VEC * chunk + e >= k_valid) { cell[e] = T(0); } }
+  }
+}
+
+// ---- epilogue ----------------------------------------------------------------------------------------------------------
+
+// V values through the layer's elementwise work: z is alpha times the sum (+ bias), `other` the residual (forward) or Z
+// (gradient). The choices are the launch's; they stand outside the loops over the values.
+template <bool FAST, int ACTIVATION, int V>
+__device__ __forceinline__ void LayerValuesOf(const LayerArgs& p, const float (&z)[V], const float (&other)[V], float (&y)[V]) {
+  if (p.gradient) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) { y[e] = z[e] * ActivationSlope<FAST>(ACTIVATION, other[e]); }
+  } else {
+#pragma unroll
+    for (int e = 0; e < V; ++e) { y[e] = Activate<FAST>(ACTIVATION, z[e]); }
+    if (p.beta != 0.0f) {
+#pragma unroll
+      for (int e = 0; e < V; ++e) { y[e] = __builtin_fmaf(p.beta, other[e], y[e]); }
+    }
+  }
+}
+template <bool FAST, int V>
+__device__ __forceinline__ void LayerValues(const LayerArgs& p, const float (&z)[V], const float (&other)[V], float (&y)[V]) {
+  switch (p.activation) {
+    case kActivationRelu: LayerValuesOf<FAST, kActivationRelu>(p, z, other, y); break;
+    case kActivationGelu: LayerValuesOf<FAST, kActivationGelu>(p, z, other, y); break;
+    case kActivationGeluTanh: LayerValuesOf<FAST, kActivationGeluTanh>(p, z, other, y); break;
+    case kActivationSilu: LayerValuesOf<FAST, kActivationSilu>(p, z, other, y); break;
+    default: LayerValuesOf<FAST, kActivationNone>(p, z, other, y); break;
+  }
+}
+
+// V consecutive values of a row, of which the first `inside` exist; WHOLE: all of them do
+template <typename T, int V>
+struct LayerPiece {
+  typedef T Piece __attribute__((ext_vector_type(V), aligned(V == 1 ? sizeof(T) : 4)));
+  static __device__ __forceinline__ void Load(const T* from, const int inside, float (&values)[V]) {
+    if (inside >= V) {
+      if constexpr (V == 1) { values[0] = static_cast<float>(*from); }
+      else {
+        const Piece piece = *reinterpret_cast<const Piece*>(from);
+#pragma unroll
+        for (int e = 0; e < V; ++e) { const T value = piece[e]; values[e] = static_cast<float>(value); }
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < V; ++e) { values[e] = (e < inside) ? static_cast<float>(from[e]) : 0.0f; }
+    }
+  }
+  static __device__ __forceinline__ void Store(T* to, const int inside, const float (&values)[V]) {
+    if (inside >= V) {
+      if constexpr (V == 1) { *to = static_cast<T>(values[0]); }
+      else {
+        Piece piece;
+#pragma unroll
+        for (int e = 0; e < V; ++e) { piece[e] = static_cast<T>(values[e]); }
+        *reinterpret_cast<Piece*>(to) = piece;
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < V; ++e) { if (e < inside) { to[e] = static_cast<T>(values[e]); } }
+    }
+  }
+};
+
+// Moves staged rows of a wavefront through the epilogue, lanes along the features in pieces of V values. The loop over
+// the rows is not unrolled (its body holds every activation); what it reads from memory is asked for two passes ahead.
+template <typename Config, int V>
+struct LayerRows {
+  using T = typename Config::T;
+  using Piece = LayerPiece<T, V>;
+  static constexpr bool FAST = sizeof(T) == 2;
+  static constexpr int PIECES = Config::WAVE_M / V;                    // of a row
+  static constexpr int ROW_LANES = PIECES < 64 ? PIECES : 64;
+  static constexpr int SETS = PIECES / ROW_LANES;                      // pieces of a row per lane
+  static constexpr int ROWS = 64 / ROW_LANES;                          // rows per pass
+  static constexpr int PASSES = Config::HALF_N / ROWS;
+  float bias[SETS][V], sums[SETS][V];
+
+  __device__ __forceinline__ void Begin(const T* bias_from, const int lane, const int inside) {
+#pragma unroll
+    for (int set = 0; set < SETS; ++set) {
+      const int col = V * (lane % ROW_LANES + set * ROW_LANES);
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        sums[set][e] = 0.0f;
+        bias[set][e] = (bias_from != nullptr && col + e < inside) ? static_cast<float>(bias_from[col + e]) : 0.0f;
+      }
+    }
+  }
+
+  // stage: the wavefront's staging tile of HALF_N rows, of which `rows` exist, each with `inside` features; c, pre, other: at
+  // the first of them
+  __device__ __forceinline__ void Run(const LayerArgs& p, const float* stage, T* c, T* pre, const T* other, const long long other_ld,
+                                      const int lane, const int rows, const int inside) {
+    constexpr int AHEAD = PASSES < 2 ? PASSES : 2;
+#pragma unroll
+    for (int set = 0; set < SETS; ++set) {
+      const int row0 = lane / ROW_LANES, col = V * (lane % ROW_LANES + set * ROW_LANES);
+      const auto inside_of = [&](const int row) { return (row < rows) ? inside - col : 0; };
+      float old[AHEAD][V];
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) { old[u][e] = 0.0f; }
+        const int row = row0 + u * ROWS;
+        if (other != nullptr) { Piece::Load(other + row * other_ld + col, inside_of(row), old[u]); }
+      }
+#pragma unroll 1
+      for (int pass = 0; pass < PASSES; pass += AHEAD) {
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+          const int row = row0 + (pass + u) * ROWS;
+          float now[V], z[V], y[V];
+#pragma unroll
+          for (int e = 0; e < V; ++e) { now[e] = old[u][e]; }
+          const int next = row + AHEAD * ROWS;
+          if (other != nullptr) { Piece::Load(other + next * other_ld + col, pass + u + AHEAD < PASSES ? inside_of(next) : 0, old[u]); }
+          const float* from = stage + row * Config::PITCH + col;
+          if constexpr (V == 1) { z[0] = *from; }
+          else {
+#pragma unroll
+            for (int q = 0; q < V; q += 4) {
+              const layer_float4_t four = *reinterpret_cast<const layer_float4_t*>(from + q);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) { z[q + e] = four[e]; }
+            }
+          }
+#pragma unroll
+          for (int e = 0; e < V; ++e) { z[e] = __builtin_fmaf(p.alpha, z[e], bias[set][e]); }
+          LayerValues<FAST>(p, z, now, y);
+          const int here = inside_of(row);
+          if (here > 0) {
+#pragma unroll
+            for (int e = 0; e < V; ++e) { sums[set][e] += y[e]; }
+          }
+          Piece::Store(c + row * p.c_ld + col, here, y);
+          if (pre != nullptr && !p.gradient) { Piece::Store(pre + row * p.pre_ld + col, here, z); }
+        }
+      }
+    }
+  }
+
+  // The wavefront's sums over its rows to `to` (LDS, WAVE_M values): lanes with the same features are added up first
+  __device__ __forceinline__ void StoreSums(float* to, const int lane) {
+#pragma unroll
+    for (int set = 0; set < SETS; ++set) {
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        float sum = sums[set][e];
+#pragma unroll
+        for (int step = ROW_LANES; step < 64; step *= 2) { sum += __shfl_xor(sum, step, 64); }
+        if (lane < ROW_LANES) { to[V * (lane + set * ROW_LANES) + e] = sum; }
+      }
+    }
+  }
+};
+
+// ---- the kernel --------------------------------------------------------------------------------------------------------
+
+template <typename Config, bool A_KC, bool B_KC>
+__global__ __launch_bounds__(Config::THREADS, Config::MIN_WAVES) void LayerGemmKernel(const LayerArgs p, const int tiles_m,
+                                                                                     const int tiles_n) {
+  using T = typename Config::T;
+  using Math = typename LayerMathOf<Config>::type;
+  using Frag = typename Math::Frag;
+  using Acc = typename Math::Acc;
+  constexpr int TILE_M = Config::TILE_M, TILE_N = Config::TILE_N, TILE_K = Config::TILE_K, BLOCK = Config::BLOCK;
+  constexpr int BM = Config::BM, BN = Config::BN, HM = BM / 2, HN = BN / 2;
+  constexpr int WAVES = Config::WAVES, ROUNDS = Config::ROUNDS, STAGES = Config::STAGES, AHEAD = STAGES - 1;
+  using KernelTag = std::tuple<Config, std::integral_constant<int, (A_KC ? 2 : 0) | (B_KC ? 1 : 0)>>;
+
+  extern __shared__ __align__(16) unsigned char lds_raw[];
+  char* a_ring = reinterpret_cast<char*>(lds_raw);
+  char* b_ring = a_ring + STAGES * Config::A_BYTES;
+  char* scratch_piece = b_ring + STAGES * Config::B_BYTES;
+
+  const int tid = threadIdx.x, lane = tid % 64;
+  const int wave = __builtin_amdgcn_readfirstlane(tid / 64);
+  const int wave_m = wave % Config::WM, wave_n = wave / Config::WM;
+
+  // ---- which tile, of which group
+  int tile_m, tile_n, group = 0;
+  int rows = p.n, depth = p.k, first = 0;  // the group's rows or depths, and where they begin
+  int sums_row;                            // the tile's row of bias_partials
+  if (p.grouping == kLayerGroupedRows) {
+    int before = 0, end = 0, index = 0;
+    const bool found = FindGroupTile(p.offsets, p.groups, p.n, TILE_N, lane, [&](const int total) {
+      const long long all = static_cast<long long>(total) * tiles_m;
+      if (static_cast<long long>(blockIdx.x) >= all || all > 0x7fffffff) { return -1; }
+      index = XcdContiguousIndex(blockIdx.x, total * tiles_m);
+      return index / tiles_m;
+    }, group, before, first, end);
+    if (!found) { return; }
+    rows = end - first;
+    // inside a group: eight tile rows of features at a time, so that the tiles in flight on an XCD share panels
+    const int group_tiles = (rows + TILE_N - 1) / TILE_N;
+    const int local = index - before * tiles_m;
+    const int walk = local / (8 * group_tiles), height = min(tiles_m - 8 * walk, 8);
+    tile_m = 8 * walk + (local - walk * 8 * group_tiles) % height;
+    tile_n = (local - walk * 8 * group_tiles) / height;
+    sums_row = before + tile_n;
+  } else if (p.grouping == kLayerGroupedDepth) {
+    const int index = XcdContiguousIndex(blockIdx.x, gridDim.x);
+    const int per_group = tiles_m * tiles_n;
+    group = index / per_group;
+    int end;
+    GroupRange(p.offsets, group, p.k, first, end);
+    depth = end - first;
+    const int local = index - group * per_group;
+    const int walk = local / (8 * tiles_n), height = min(tiles_m - 8 * walk, 8);
+    tile_m = 8 * walk + (local - walk * 8 * tiles_n) % height;
+    tile_n = (local - walk * 8 * tiles_n) / height;
+    sums_row = tile_n;
+  } else {
+    TileOfBlock<(TILE_M >= 2 * TILE_N) ? 4 : 8>(blockIdx.x, gridDim.x, tiles_m, tiles_n, tile_m, tile_n);
+    sums_row = tile_n;
+    if (p.split_chunk > 0) {
+      first = blockIdx.y * p.split_chunk;
+      depth = min(p.split_chunk, p.k - first);
+    }
+  }
+  const int m0 = tile_m * TILE_M, n0 = tile_n * TILE_N;
+  const T* a = static_cast<const T*>(p.a);
+  const T* b = static_cast<const T*>(p.b);
+  if (p.grouping == kLayerGroupedRows) {
+    a += group * p.a_stride;
+    b += first * (B_KC ? p.b_ld : 1);
+  } else {  // (first is 0 but for K ranges and groups by depth)
+    a += first * (A_KC ? 1 : p.a_ld);
+    b += first * (B_KC ? 1 : p.b_ld);
+  }
+
+  Acc acc[BM][BN];
+#pragma unroll
+  for (int i = 0; i < BM; ++i) {
+#pragma unroll
+    for (int j = 0; j < BN; ++j) { acc[i][j] = Acc(0.0f); }
+  }
+
+  const int slabs = (depth + TILE_K - 1) / TILE_K;
+  const int k_tail = depth % TILE_K;
+  if (slabs > 0) {
+    int a_offset[BM], b_offset[BN];
+#pragma unroll
+    for (int q = 0; q < BM; ++q) { a_offset[q] = Math::template Offset<TILE_M, A_KC>(lane, (wave_m * BM + q) * BLOCK); }
+#pragma unroll
+    for (int q = 0; q < BN; ++q) { b_offset[q] = Math::template Offset<TILE_N, B_KC>(lane, (wave_n * BN + q) * BLOCK); }
+    const auto read_a = [&](const char* stage, const int q) {
+      if constexpr (sizeof(T) == 4) { return Math::template Read<TILE_M, A_KC>(stage, a_offset[q], lane); }
+      else { return Math::template Read<TILE_M, A_KC>(stage, a_offset[q]); }
+    };
+    const auto read_b = [&](const char* stage, const int q) {
+      if constexpr (sizeof(T) == 4) { return Math::template Read<TILE_N, B_KC>(stage, b_offset[q], lane); }
+      else { return Math::template Read<TILE_N, B_KC>(stage, b_offset[q]); }
+    };
+
+    constexpr long long SIZE = sizeof(T);
+    const char* a_tile = reinterpret_cast<const char*>(a + (A_KC ? m0 * p.a_ld : static_cast<long long>(m0)));
+    const char* b_tile = reinterpret_cast<const char*>(b + (B_KC ? n0 * p.b_ld : static_cast<long long>(n0)));
+    // behind the last element of the operand
+    const char* a_end = reinterpret_cast<const char*>(a + (A_KC ? (p.m - 1) * p.a_ld + depth : (depth - 1) * p.a_ld + p.m));
+    const char* b_end = reinterpret_cast<const char*>(b + (B_KC ? (rows - 1) * p.b_ld + depth : (depth - 1) * p.b_ld + rows));
+
+    auto walk = [&](auto range_tag) {
+      constexpr bool RANGE = decltype(range_tag)::value;
+      const char* a_request = a_tile;  // first line of the slab to be requested next
+      const char* b_request = b_tile;
+      const long long a_step = A_KC ? 64 : TILE_K * p.a_ld * SIZE;
+      const long long b_step = B_KC ? 64 : TILE_K * p.b_ld * SIZE;
+      constexpr int A_LINES = A_KC ? 16 : 1024 / (TILE_M * static_cast<int>(SIZE));
+      constexpr int B_LINES = B_KC ? 16 : 1024 / (TILE_N * static_cast<int>(SIZE));
+      const auto is_a = [&](const int round, const int piece) {
+        return (Config::PIECES_A % WAVES == 0) ? (round < Config::PIECES_A / WAVES) : (piece < Config::PIECES_A);
+      };
+      long long piece_start[ROUNDS];
+      int piece_lane_bytes[ROUNDS], piece_place[ROUNDS];
+#pragma unroll
+      for (int round = 0; round < ROUNDS; ++round) {
+        const int piece = wave + WAVES * round;
+        if (is_a(round, piece)) {
+          piece_start[round] = static_cast<long long>(A_LINES * piece) * p.a_ld * SIZE;
+          piece_lane_bytes[round] = LayerPieceLaneBytes<T, TILE_M, A_KC>(p.a_ld, piece, lane);
+          piece_place[round] = piece * 1024;
+        } else {
+          const int b_piece = piece - Config::PIECES_A;
+          piece_start[round] = static_cast<long long>(B_LINES * b_piece) * p.b_ld * SIZE;
+          piece_lane_bytes[round] = LayerPieceLaneBytes<T, TILE_N, B_KC>(p.b_ld, b_piece, lane);
+          piece_place[round] = b_piece * 1024;
+        }
+      }
+      const auto request = [&](const int round, const int buffer) {
+        const int piece = wave + WAVES * round;
+        if (is_a(round, piece)) {
+          char* place = a_ring + buffer * Config::A_BYTES + piece_place[round];
+          LayerRequestPiece<RANGE, KernelTag>(a_request + piece_start[round], a_end, place, piece_lane_bytes[round]);
+        } else if (!Config::DUMMY || piece < Config::PIECES_A + Config::PIECES_B) {
+          char* place = b_ring + buffer * Config::B_BYTES + piece_place[round];
+          LayerRequestPiece<RANGE, KernelTag>(b_request + piece_start[round], b_end, place, piece_lane_bytes[round]);
+        } else {
+          // keeps the number of requests in flight equal in all wavefronts (the waits count them): moves nothing
+          LayerRequestPiece<true, KernelTag>(a_tile, a_tile, scratch_piece, lane * 16);
+        }
+      };
+      const auto zero_tail = [&](const int buffer) {
+        if (!RANGE || k_tail == 0 || !(A_KC || B_KC)) { return; }
+#pragma unroll
+        for (int round = 0; round < ROUNDS; ++round) {
+          const int piece = wave + WAVES * round;
+          if (piece < Config::PIECES_A) {
+            if (A_KC) { LayerZeroTail<T>(a_ring + buffer * Config::A_BYTES, piece, lane, k_tail); }
+          } else if (piece < Config::PIECES_A + Config::PIECES_B) {
+            if (B_KC) { LayerZeroTail<T>(b_ring + buffer * Config::B_BYTES, piece - Config::PIECES_A, lane, k_tail); }
+          }
+        }
+      };
+
+      const int first_slabs = min(slabs, AHEAD);
+#pragma unroll
+      for (int s = 0; s < AHEAD; ++s) {
+        if (s < first_slabs) {
+#pragma unroll
+          for (int round = 0; round < ROUNDS; ++round) { request(round, s); }
+          a_request += a_step;
+          b_request += b_step;
+        }
+      }
+      if (first_slabs == 1) { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+      else { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(ROUNDS) : "memory"); }
+      if (slabs == 1) { zero_tail(0); }
+      __syncthreads();
+      Frag a_frag[2][HM], b_frag[2][HN];
+#pragma unroll
+      for (int q = 0; q < HM; ++q) { a_frag[0][q] = read_a(a_ring, q); }
+#pragma unroll
+      for (int q = 0; q < HN; ++q) { b_frag[0][q] = read_b(b_ring, q); }
+      int cur = 0;
+      // One slab; LATER: how many follow it, capped at AHEAD. Slab + 2 is requested under the first two quadrants, into the
+      // buffer whose reads everybody had waited for at the previous barrier.
+      constexpr int PER_SLOT = (ROUNDS + 2 * HM - 1) / (2 * HM);
+      const auto slab_body = [&](auto later_tag) {
+        constexpr int LATER = decltype(later_tag)::value;
+        constexpr bool LOAD = LATER == AHEAD;
+        const int nxt = (cur == STAGES - 1) ? 0 : cur + 1, prv = (cur == 0) ? STAGES - 1 : cur - 1;
+        const char* a_cur = a_ring + cur * Config::A_BYTES;
+        const char* b_cur = b_ring + cur * Config::B_BYTES;
+        const char* a_nxt = a_ring + nxt * Config::A_BYTES;
+        const char* b_nxt = b_ring + nxt * Config::B_BYTES;
+#pragma unroll
+        for (int quadrant = 0; quadrant < 4; ++quadrant) {
+          const int ha = quadrant / 2, hb = quadrant % 2;
+#pragma unroll
+          for (int q = 0; q < HM; ++q) {
+            if (quadrant == 0 || quadrant == 3) {
+              if (q < HN) {
+                if (quadrant == 0) { b_frag[1][q] = read_b(b_cur, HN + q); }
+                else { b_frag[0][q] = read_b(b_nxt, q); }
+              }
+            } else if (quadrant == 1) {
+              a_frag[1][q] = read_a(a_cur, HM + q);
+            } else {
+              a_frag[0][q] = read_a(a_nxt, q);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int j = 0; j < HN; ++j) {
+              acc[ha * HM + q][hb * HN + j] = Math::Multiply(a_frag[ha][q], b_frag[hb][j], acc[ha * HM + q][hb * HN + j]);
+            }
+            if (LOAD && quadrant < 2) {
+#pragma unroll
+              for (int u = 0; u < PER_SLOT; ++u) {
+                const int round = (quadrant * HM + q) * PER_SLOT + u;
+                if (round < ROUNDS) { request(round, prv); }
+              }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+          }
+          if (quadrant == 1) {
+            // slab + 1 must have landed for everybody; the requests for the slab behind it may stay in flight
+            constexpr int IN_FLIGHT = (LATER >= 2) ? ROUNDS : 0;
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(IN_FLIGHT) : "memory");
+            if (LATER == 1) { zero_tail(nxt); }  // slab + 1 is the last one
+            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+          }
+        }
+        cur = nxt;
+        if (LOAD) {
+          a_request += a_step;
+          b_request += b_step;
+        }
+      };
+      int slab = 0;
+      for (; slab + AHEAD < slabs; ++slab) { slab_body(std::integral_constant<int, AHEAD>{}); }
+      if (slab + 1 < slabs) { slab_body(std::integral_constant<int, 1>{}); ++slab; }
+      slab_body(std::integral_constant<int, 0>{});
+    };
+    if (m0 + TILE_M <= p.m && n0 + TILE_N <= rows && k_tail == 0) { walk(std::false_type{}); }
+    else { walk(std::true_type{}); }
+  }
+
+  // ---- K ranges: the sums as they are
+  if (p.split_chunk > 0) {
+    float* partial = p.partials + static_cast<long long>(blockIdx.y) * p.n * p.m;
+#pragma unroll
+    for (int j = 0; j < BN; ++j) {
+      const int row = n0 + (wave_n * BN + j) * BLOCK + lane % BLOCK;
+#pragma unroll
+      for (int i = 0; i < BM; ++i) {
+#pragma unroll
+        for (int r = 0; r < static_cast<int>(sizeof(Acc) / 16); ++r) {
+          const int col = m0 + (wave_m * BM + i) * BLOCK + (BLOCK == 32 ? 8 * r + 4 * (lane / 32) : 4 * (lane / 16));
+          float* to = partial + static_cast<long long>(row) * p.m + col;
+          if (row < p.n) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) { if (col + e < p.m) { to[e] = acc[i][j][4 * r + e]; } }
+          }
+        }
+      }
+    }
+    return;
+  }
+
+  // ---- epilogue
+  __syncthreads();  // every wavefront is done with the slab buffers
+  int late_lane = lane;  // (opaque, so that what the epilogue derives from it does not occupy registers during the walk)
+  asm volatile("" : "+v"(late_lane));
+  float* stage = reinterpret_cast<float*>(lds_raw + wave * Config::STAGE_BYTES);
+  float* tile_sums = reinterpret_cast<float*>(lds_raw + Config::EPILOGUE_BYTES);
+  const int wave_m0 = m0 + wave_m * Config::WAVE_M;
+  const int inside = p.m - wave_m0;
+  const long long first_row = (p.grouping == kLayerGroupedRows) ? first : 0;
+  T* c = static_cast<T*>(p.c) + first_row * p.c_ld + ((p.grouping == kLayerGroupedDepth) ? group * p.c_stride : 0) + wave_m0;
+  T* pre = (p.pre == nullptr) ? nullptr : static_cast<T*>(p.pre) + first_row * p.pre_ld + wave_m0;
+  const T* other = nullptr;
+  long long other_ld = 0;
+  if (p.gradient) {
+    other = pre;
+    other_ld = p.pre_ld;
+  } else if (p.beta != 0.0f) {
+    // (of groups by depth the residual is C itself, in place)
+    other = static_cast<const T*>(p.residual) + first_row * p.residual_ld +
+            ((p.grouping == kLayerGroupedDepth) ? group * p.c_stride : 0) + wave_m0;
+    other_ld = p.residual_ld;
+  }
+  const T* bias = (p.bias == nullptr) ? nullptr : static_cast<const T*>(p.bias) + group * p.bias_stride + wave_m0;
+  const auto wave_fence = [&]() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  };
+  const auto finish = [&](auto rows_of) {
+    if (inside > 0) {
+      rows_of.Begin(bias, late_lane, inside);
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+#pragma unroll
+        for (int j = 0; j < HN; ++j) {
+#pragma unroll
+          for (int i = 0; i < BM; ++i) {
+#pragma unroll
+            for (int r = 0; r < static_cast<int>(sizeof(Acc) / 16); ++r) {
+              const int col = i * BLOCK + (BLOCK == 32 ? 8 * r + 4 * (late_lane / 32) : 4 * (late_lane / 16));
+              layer_float4_t run;
+#pragma unroll
+              for (int e = 0; e < 4; ++e) { run[e] = acc[i][half * HN + j][4 * r + e]; }
+              *reinterpret_cast<layer_float4_t*>(&stage[(j * BLOCK + late_lane % BLOCK) * Config::PITCH + col]) = run;
+            }
+          }
+        }
+        wave_fence();
+        const int n_block = n0 + wave_n * Config::WAVE_N + half * Config::HALF_N;
+        if (n_block < rows) {
+          rows_of.Run(p, stage, c + n_block * p.c_ld, (pre == nullptr) ? nullptr : pre + n_block * p.pre_ld,
+                      (other == nullptr) ? nullptr : other + n_block * other_ld, other_ld, late_lane, rows - n_block, inside);
+        }
+        wave_fence();
+      }
+      if (p.bias_partials != nullptr) { rows_of.StoreSums(tile_sums + wave_n * TILE_M + wave_m * Config::WAVE_M, late_lane); }
+    }
+  };
+  if (p.vector_rows) { finish(LayerRows<Config, Config::VEC>{}); }
+  else { finish(LayerRows<Config, 1>{}); }
+  if (p.bias_partials != nullptr) {
+    __syncthreads();
+    for (int i = tid; i < TILE_M && m0 + i < p.m; i += Config::THREADS) {
+      float sum = tile_sums[i];
+#pragma unroll
+      for (int w = 1; w < Config::WN; ++w) { sum += tile_sums[w * TILE_M + i]; }
+      p.bias_partials[static_cast<long long>(sums_row) * p.m + m0 + i] = sum;
+    }
+  }
+}
+
+}  // namespace clbh
+
+#endif  // CLBLAST_HIP_KERNELS_LAYER_GEMM_HPP_

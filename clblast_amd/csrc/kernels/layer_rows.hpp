@@ -1,0 +1,186 @@
+// =================================================================================================
+// The elementwise work of a layer without a product of its own, and column sums:
+//   * LayerRowsKernel: the epilogue of kernels/layer_gemm.hpp on sums that are already there - the fp32 sums of a product
+//     whose K range was split over several work-groups (added up here in the order of the ranges), or, for the gradient of
+//     an activation, a matrix of the caller's. One pass over memory; bound by it.
+//   * LayerColumnSumsKernel: the second half of a bias gradient, which adds up the sums that the work-groups of either
+//     kernel left for their tiles of rows, in the order of the tiles: the result does not depend on timing.
+// =================================================================================================
+#ifndef CLBLAST_HIP_KERNELS_LAYER_ROWS_HPP_
+#define CLBLAST_HIP_KERNELS_LAYER_ROWS_HPP_
+
+#include "kernels/layer_gemm.hpp"
+
+namespace clbh {
+
+constexpr int kLayerRowsThreads = 256;
+
+struct LayerRowsArgs {
+  LayerArgs layer;       // c (nullptr: only the column sums are wanted), pre, residual, bias, alpha, beta, groups, ...
+  const void* upstream;  // of the storage type, or nullptr: the fp32 sums at layer.partials
+  long long upstream_ld;
+  int ranges;            // K ranges at layer.partials
+  int chunk;             // rows per work-group
+  int column_blocks;     // work-groups side by side; the grid's only dimension counts them first
+};
+
+// Work-group: 64 pieces of V features (lanes) times `chunk` rows, which its four wavefronts take in turn; four rows of a
+// wavefront are in flight at a time. bias_partials: one row of m sums for every chunk, the chunks numbered through the groups.
+template <typename T, int V>
+__global__ __launch_bounds__(kLayerRowsThreads) void LayerRowsKernel(const LayerRowsArgs q) {
+  constexpr bool FAST = sizeof(T) == 2;
+  constexpr int WAVES = kLayerRowsThreads / 64, FLIGHT = 4;
+  typedef float Four __attribute__((ext_vector_type(4), aligned(4)));
+  const LayerArgs& p = q.layer;
+  __shared__ float wave_sums[WAVES][64 * V];
+  const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  const int column_block = blockIdx.x % q.column_blocks;
+  const int col = (column_block * 64 + lane) * V;
+  const int inside = p.m - col;  // features from this lane's first one on
+  const bool whole = inside >= V;
+
+  const int sums_row = blockIdx.x / q.column_blocks;
+  int first, end;
+  if (p.grouping == kLayerGroupedRows) {
+    int group = 0, before = 0, begin = 0, last = 0;
+    if (!FindGroupTile(p.offsets, p.groups, p.n, q.chunk, lane, [&](int) { return sums_row; }, group, before, begin, last)) { return; }
+    first = begin + (sums_row - before) * q.chunk;
+    end = min(first + q.chunk, last);
+  } else {
+    first = sums_row * q.chunk;
+    end = min(first + q.chunk, p.n);
+  }
+
+  float bias[V], sums[V];
+#pragma unroll
+  for (int e = 0; e < V; ++e) {
+    sums[e] = 0.0f;
+    bias[e] = (p.bias != nullptr && e < inside) ? static_cast<float>(static_cast<const T*>(p.bias)[col + e]) : 0.0f;
+  }
+  const T* other = p.gradient ? static_cast<const T*>(p.pre) : ((p.beta != 0.0f) ? static_cast<const T*>(p.residual) : nullptr);
+  const long long other_ld = p.gradient ? p.pre_ld : p.residual_ld;
+  const auto load_sums = [&](const float* from, float* values) {
+    if (whole) {
+      if constexpr (V == 1) { values[0] = *from; }
+      else {
+#pragma unroll
+        for (int h = 0; h < V; h += 4) {
+          const Four four = *reinterpret_cast<const Four*>(from + h);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) { values[h + e] = four[e]; }
+        }
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < V; ++e) { values[e] = (e < inside) ? from[e] : 0.0f; }
+    }
+  };
+  if (inside > 0) {
+    for (int row0 = first + wave; row0 < end; row0 += WAVES * FLIGHT) {
+      float z[FLIGHT][V], old[FLIGHT][V];
+#pragma unroll
+      for (int u = 0; u < FLIGHT; ++u) {
+        const long long row = min(row0 + WAVES * u, end - 1);  // (a row beyond the chunk: the last one again, not used)
+        if (q.upstream != nullptr) { LayerPiece<T, V>::Load(static_cast<const T*>(q.upstream) + row * q.upstream_ld + col, inside, z[u]); }
+        else { load_sums(p.partials + row * p.m + col, z[u]); }
+        if (other != nullptr) { LayerPiece<T, V>::Load(other + row * other_ld + col, inside, old[u]); }
+        else {
+#pragma unroll
+          for (int e = 0; e < V; ++e) { old[u][e] = 0.0f; }
+        }
+      }
+      for (int range = 1; range < q.ranges; ++range) {
+        const float* slab = p.partials + static_cast<long long>(range) * p.n * p.m;
+        float more[FLIGHT][V];
+#pragma unroll
+        for (int u = 0; u < FLIGHT; ++u) {
+          const long long row = min(row0 + WAVES * u, end - 1);
+          load_sums(slab + row * p.m + col, more[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < FLIGHT; ++u) {
+#pragma unroll
+          for (int e = 0; e < V; ++e) { z[u][e] += more[u][e]; }
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < FLIGHT; ++u) {
+        const long long row = row0 + WAVES * u;
+        if (row < end) {
+          float y[V];
+#pragma unroll
+          for (int e = 0; e < V; ++e) { z[u][e] = __builtin_fmaf(p.alpha, z[u][e], bias[e]); }
+          LayerValues<FAST>(p, z[u], old[u], y);
+#pragma unroll
+          for (int e = 0; e < V; ++e) { sums[e] += y[e]; }
+          if (p.c != nullptr) { LayerPiece<T, V>::Store(static_cast<T*>(p.c) + row * p.c_ld + col, inside, y); }
+          if (p.pre != nullptr && !p.gradient) { LayerPiece<T, V>::Store(static_cast<T*>(p.pre) + row * p.pre_ld + col, inside, z[u]); }
+        }
+      }
+    }
+  }
+  if (p.bias_partials != nullptr) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) { wave_sums[wave][lane * V + e] = sums[e]; }
+    __syncthreads();
+    for (int i = threadIdx.x; i < 64 * V; i += kLayerRowsThreads) {
+      const int feature = column_block * 64 * V + i;
+      if (feature < p.m) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) { sum += wave_sums[w][i]; }
+        p.bias_partials[static_cast<long long>(sums_row) * p.m + feature] = sum;
+      }
+    }
+  }
+}
+
+// out[group * out_stride + i] = the sum of the group's rows of `partials` (m values each): with offsets the tiles of `tile`
+// rows that the groups are cut into, numbered through from group 0 on; without, all `rows_of_sums` rows. Zero for a
+// group without a tile. grid: (ceil(m / 64), groups); the four wavefronts take every fourth row.
+template <typename T>
+__global__ __launch_bounds__(kLayerRowsThreads) void LayerColumnSumsKernel(const float* __restrict__ partials, const int rows_of_sums,
+                                                                           const int m, const long long* __restrict__ offsets,
+                                                                           const int groups, const int rows, const int tile,
+                                                                           T* __restrict__ out, const long long out_stride) {
+  constexpr int WAVES = kLayerRowsThreads / 64;
+  __shared__ float wave_sums[WAVES][64];
+  const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  for (int group = blockIdx.y; group < groups; group += gridDim.y) {
+    int first = 0, count = rows_of_sums;
+    if (offsets != nullptr) {  // tiles of the groups in front of this one, and of this one
+      int before = 0;
+      for (int g = lane; g < group; g += 64) {
+        const long long from = offsets[g], to = offsets[g + 1];
+        const int begin = static_cast<int>(from < 0 ? 0 : (from > rows ? rows : from));
+        const int size = static_cast<int>(to < begin ? 0 : (to > rows ? rows : to) - begin);
+        before += (size + tile - 1) / tile;
+      }
+#pragma unroll
+      for (int step = 32; step >= 1; step /= 2) { before += __shfl_xor(before, step, 64); }
+      int begin, end;
+      GroupRange(offsets, group, rows, begin, end);
+      first = min(before, rows_of_sums);
+      count = min((end - begin + tile - 1) / tile, rows_of_sums - first);
+    }
+    const int feature = blockIdx.x * 64 + lane;
+    float sum = 0.0f;
+    if (feature < m) {
+      const float* from = partials + static_cast<long long>(first) * m + feature;
+#pragma unroll 8
+      for (int t = wave; t < count; t += WAVES) { sum += from[static_cast<long long>(t) * m]; }
+    }
+    wave_sums[wave][lane] = sum;
+    __syncthreads();
+    if (wave == 0 && feature < m) {
+#pragma unroll
+      for (int w = 1; w < WAVES; ++w) { sum += wave_sums[w][lane]; }
+      out[group * out_stride + feature] = static_cast<T>(sum);
+    }
+    __syncthreads();
+  }
+}
+
+}  // namespace clbh
+
+#endif  // CLBLAST_HIP_KERNELS_LAYER_ROWS_HPP_

@@ -8,6 +8,7 @@
 #include <map>
 #include <mutex>
 #include <tuple>
+#include <utility>
 
 #include "clbh_device.h"
 
@@ -19,6 +20,8 @@ std::map<std::tuple<int, int>, size_t> min_indirect_overrides;  // (device, prec
 std::map<int, size_t> tile_variant_overrides;                   // precision bits -> forced MFMA tile (0 = automatic)
 std::map<int, size_t> split_overrides;                          // precision bits -> K ranges of a forced tile
 std::map<int, size_t> conv_slab_overrides;                      // precision bits -> 1: CONVGEMM's slab kernel whenever possible, 2: never
+
+std::map<int, std::pair<size_t, size_t>> layer_overrides;       // precision bits -> (tile of the layer products, K ranges)
 
 size_t ForcedSplit(const Precision precision) {
   std::lock_guard<std::mutex> lock(override_mutex);
@@ -755,6 +758,15 @@ bool UseConvSlab(const Precision precision, const size_t taps, const size_t kern
   return use >= 0.65;
 }
 
+void ApplyLayerOverrides(const Precision precision, int& tile_variant, int& split_k) {
+  std::lock_guard<std::mutex> lock(override_mutex);
+  if (layer_overrides.empty()) { return; }
+  const auto found = layer_overrides.find(static_cast<int>(precision));
+  if (found == layer_overrides.end()) { return; }
+  if (found->second.first > 0 && found->second.first < 100) { tile_variant = static_cast<int>(found->second.first) - 1; }
+  if (found->second.second < 65536) { split_k = static_cast<int>(found->second.second); }
+}
+
 StatusCode OverrideRoutineParameters(const int device, const std::string& kernel_name, const Precision precision,
                                      const std::unordered_map<std::string, size_t>& parameters) {
   if (kernel_name == "Xconvgemm") {  // SLAB: 0 = by rule, 1 = the slab kernel whenever it can run, 2 = never
@@ -764,6 +776,17 @@ StatusCode OverrideRoutineParameters(const int device, const std::string& kernel
     }
     std::lock_guard<std::mutex> lock(override_mutex);
     conv_slab_overrides[static_cast<int>(precision)] = slab->second;
+    return StatusCode::kSuccess;
+  }
+  if (kernel_name == "Xlayer") {  // the layer products: TILE_VARIANT = 1 + index, SPLIT_K = K ranges, 0 = automatic
+    const auto variant = parameters.find("TILE_VARIANT");
+    if (variant == parameters.end()) {
+      return StatusCode::kMissingOverrideParameter;
+    }
+    const auto split = parameters.find("SPLIT_K");
+    std::lock_guard<std::mutex> lock(override_mutex);
+    layer_overrides[static_cast<int>(precision)] =
+        std::make_pair(variant->second, (split != parameters.end()) ? split->second : size_t{0});
     return StatusCode::kSuccess;
   }
   if (kernel_name == "Xgemm") {  // forces one tile of the MFMA family: TILE_VARIANT = 1 + index, 0 = automatic
@@ -797,6 +820,13 @@ StatusCode RetrieveRoutineParameters(const int device, const std::string& kernel
     parameters["SLAB"] = (found != conv_slab_overrides.end()) ? found->second : 0;
     return StatusCode::kSuccess;
   }
+  if (kernel_name == "Xlayer") {
+    std::lock_guard<std::mutex> lock(override_mutex);
+    const auto found = layer_overrides.find(static_cast<int>(precision));
+    parameters["TILE_VARIANT"] = (found != layer_overrides.end()) ? found->second.first : 0;
+    parameters["SPLIT_K"] = (found != layer_overrides.end()) ? found->second.second : 0;
+    return StatusCode::kSuccess;
+  }
   if (kernel_name == "Xgemm") {
     parameters["TILE_VARIANT"] = ForcedTileVariant(precision);
     parameters["SPLIT_K"] = ForcedSplit(precision);
@@ -815,6 +845,7 @@ void ClearOverrides() {
   tile_variant_overrides.clear();
   split_overrides.clear();
   conv_slab_overrides.clear();
+  layer_overrides.clear();
 }
 
 }  // namespace clblast

@@ -51,6 +51,11 @@ size_t ForcedTileVariant(const Precision precision);
 bool UseConvSlab(const Precision precision, const size_t taps, const size_t kernels, const size_t work_groups,
                  const size_t tile_pixels, const size_t tile_kernels, const size_t compute_units);
 
+// The layer products (GemmEpilogue, GemmGrouped, ...): a tile and a number of K ranges forced through
+// OverrideParameters("Xlayer", {"TILE_VARIANT": 1 + index, "SPLIT_K": ranges}); leaves the arguments alone where nothing is
+// forced. Precision kHalf stands for both 16-bit types.
+void ApplyLayerOverrides(const Precision precision, int& tile_variant, int& split_k);
+
 // Parameter override store behind clblast::OverrideParameters / RetrieveParameters / ClearCache.
 StatusCode OverrideRoutineParameters(const int device, const std::string& kernel_name, const Precision precision,
                                      const std::unordered_map<std::string, size_t>& parameters);

@@ -259,6 +259,63 @@ CLBH_API int clbh_conv_slab(int precision, const clbh_im2col_shape* shape, int k
                             long long images_offset, const void* weights, long long weights_offset, void* result,
                             long long result_offset, void* scratch, hipStream_t stream);
 
+// ---- products of a network's layers (kernels/layer_gemm.hpp) ---------------------------------------------------------
+// Canonical problem as for clbh_gemm_desc - C(i,j) for i < m features (contiguous in C) and j < n rows, A the weights, B the
+// rows - with the layer's elementwise work behind it:
+//   gradient == 0:  Z = alpha * A * B + bias(i),  C = act(Z) + beta * residual(i,j);  Z is also stored at `pre`, unless NULL
+//   gradient != 0:  C = alpha * A * B * act'(Z(i,j)), Z read at `pre`; bias_gradient(i) = sum over j of C(i,j), unless NULL
+// (the sum is taken before C is rounded). upstream != NULL: that matrix (leading dimension upstream_ld) stands in place of
+// A * B, there is no product, and c may be NULL where only the sums are wanted (with activation none `pre` may be, too).
+// Groups: offsets is a device array of groups + 1 ascending values. By rows: group g owns the rows offsets[g] ..
+// offsets[g+1] - 1 and has A at a + g * a_stride, bias at bias + g * bias_stride, bias_gradient at bias_gradient + g * m;
+// needs b_kcontig. Rows of no group are neither read nor written. By depth: group g owns that range of k, C at c +
+// g * c_stride; needs both operands x-contiguous. Values outside 0 .. n (0 .. k) are clamped.
+// All pointers are those of the first element. residual is not read when beta == 0; it may be C itself.
+#define CLBH_TYPE_FP16 16
+#define CLBH_TYPE_FP32 32
+#define CLBH_TYPE_BF16 1600
+#define CLBH_GROUPS_NONE 0
+#define CLBH_GROUPS_BY_ROWS 1
+#define CLBH_GROUPS_BY_DEPTH 2
+#define CLBH_LAYER_MAX_LD (1ll << 23)        // operands: 16 lines of a slab stay at 32-bit byte offsets
+#define CLBH_LAYER_MAX_GROUPED (1ll << 26)   // rows (depths) of a grouped call
+#define CLBH_LAYER_MAX_GROUPS (1ll << 20)
+typedef struct clbh_layer_desc_ {
+  int type;          // CLBH_TYPE_...
+  int tile_variant;  // index into kLayerTiles (device/layer_plans.hpp), -1: chosen by size
+  int split_k;       // K ranges of a product without groups, 0: chosen by size
+  int a_kcontig, b_kcontig;
+  int m, n, k;
+  float alpha, beta;
+  const void* a;
+  const void* b;
+  void* c;
+  long long a_ld, b_ld, c_ld;
+  long long a_stride, c_stride;
+  const void* bias;
+  long long bias_stride;
+  void* pre;
+  long long pre_ld;
+  const void* residual;
+  long long residual_ld;
+  int activation;    // 161 none, 162 relu, 163 gelu, 164 gelu (tanh form), 165 silu
+  int gradient;
+  void* bias_gradient;
+  const void* upstream;
+  long long upstream_ld;
+  int grouping;      // CLBH_GROUPS_...
+  int groups;
+  const long long* offsets;
+  void* workspace;   // clbh_layer_workspace_bytes(desc) bytes, 256-byte aligned
+  size_t workspace_bytes;
+} clbh_layer_desc;
+// 16-bit operands are fetched in dwords: 1 when a and b can be (dword-aligned, even leading dimensions and strides, leading
+// dimensions below CLBH_LAYER_MAX_LD), 0 when the caller has to copy the operand that cannot (bit 0: a, bit 1: b of *copy).
+CLBH_API int clbh_layer_operands_fit(const clbh_layer_desc* desc, int* copy);
+CLBH_API size_t clbh_layer_workspace_bytes(const clbh_layer_desc* desc);
+// Enqueues the kernels of one call. Returns 0 or the HIP error code.
+CLBH_API int clbh_layer_launch(const clbh_layer_desc* desc, hipStream_t stream);
+
 // Plain device memory and blocking copies for callers that hold host data (the Netlib-style façade): to_device != 0
 // copies host -> device, else waits for the default stream's work and copies device -> host.
 CLBH_API int clbh_alloc(void** ptr, size_t bytes);

@@ -103,10 +103,14 @@ enum class Triangle { kUpper = 121, kLower = 122 };
 enum class Diagonal { kNonUnit = 131, kUnit = 132 };
 enum class Side { kLeft = 141, kRight = 142 };
 enum class KernelMode { kCrossCorrelation = 151, kConvolution = 152 };
+// Activations of the layer products (GemmEpilogue, ...): kGelu is z Phi(z), kGeluTanh its tanh form, kSilu z / (1 + exp(-z))
+enum class Activation { kNone = 161, kRelu = 162, kGelu = 163, kGeluTanh = 164, kSilu = 165 };
 enum class Precision { kHalf = 16, kSingle = 32, kDouble = 64, kComplexSingle = 3232, kComplexDouble = 6464, kAny = -1 };
 
 // Host type of fp16 scalars and data: the IEEE binary16 bit pattern (reference: clblast_half.h:21).
 using half = unsigned short;
+// Host type of bfloat16 data: the upper half of an IEEE binary32 (layer products only).
+struct bfloat16 { unsigned short bits; };
 // Complex scalars and data, interleaved (real, imaginary) (reference: src/utilities/utilities.hpp:33-35).
 using float2 = std::complex<float>;
 using double2 = std::complex<double>;
@@ -230,6 +234,74 @@ StatusCode Convgemm(const KernelMode kernel_mode, const size_t channels, const s
                     const size_t num_kernels, const size_t batch_count, const void* im_buffer, const size_t im_offset,
                     const void* kernel_buffer, const size_t kernel_offset, void* result_buffer,
                     const size_t result_offset, hipStream_t* queue, hipEvent_t* event = nullptr);
+
+// ---- Products of a network's layers ------------------------------------------------------------------------------------
+// T is float, half or bfloat16; sums, scalars and the elementwise work are in 32 bits, every result is rounded once. All
+// matrices are row-major (a column-major caller exchanges A and B, and m and n); offsets, leading dimensions and strides
+// are in elements. The reference has no such routines. Zero sizes return kInvalidDimension, a group count of zero kInvalidBatchCount;
+// the codes of `pre` and `residual` are those of matrix C, the codes of `bias` and `bias_gradient` those of vector X, the
+// codes of `group_offsets` those of vector Y.
+
+// Z = alpha * op(A) * op(B) + bias, C = act(Z) + beta * R, for op(A) m x k, op(B) k x n and a bias of n values that every row
+// gets (nullptr: none). Z (m x n) is stored at `pre` as well unless that is nullptr; activation kNone makes this a
+// product with bias and residual. The residual R (m x n) is not read when beta is zero; it may be C itself.
+template <typename T>
+StatusCode GemmEpilogue(const Transpose a_transpose, const Transpose b_transpose, const size_t m, const size_t n,
+                        const size_t k, const float alpha, const void* a_buffer, const size_t a_offset, const size_t a_ld,
+                        const void* b_buffer, const size_t b_offset, const size_t b_ld, const void* bias_buffer,
+                        const size_t bias_offset, const Activation activation, void* pre_buffer, const size_t pre_offset,
+                        const size_t pre_ld, const float beta, const void* residual_buffer, const size_t residual_offset,
+                        const size_t residual_ld, void* c_buffer, const size_t c_offset, const size_t c_ld,
+                        hipStream_t* queue, hipEvent_t* event = nullptr);
+
+// C = (alpha * op(A) * op(B)) . act'(Z), element by element with the Z that GemmEpilogue stored at `pre` (not read for kNone),
+// and bias_gradient(j) = the sum of column j of C (before its rounding; always in the same order) unless that is nullptr: the
+// backward pass of a product through the activation in front of it. The gradients of the operands are products of C.
+template <typename T>
+StatusCode GemmActivationGradient(const Transpose a_transpose, const Transpose b_transpose, const size_t m, const size_t n,
+                                  const size_t k, const float alpha, const void* a_buffer, const size_t a_offset,
+                                  const size_t a_ld, const void* b_buffer, const size_t b_offset, const size_t b_ld,
+                                  const Activation activation, const void* pre_buffer, const size_t pre_offset,
+                                  const size_t pre_ld, void* c_buffer, const size_t c_offset, const size_t c_ld,
+                                  void* bias_gradient_buffer, const size_t bias_gradient_offset, hipStream_t* queue,
+                                  hipEvent_t* event = nullptr);
+
+// The same where the gradient comes from elsewhere: C = Y . act'(Z) for m x n matrices, C may be Y itself. C may be nullptr
+// where only the sums are wanted. With groups (group_offsets not nullptr, see GemmGrouped) only their rows take part, and
+// bias_gradient holds group_count vectors of n values, one behind the other (zeros for a group without rows).
+template <typename T>
+StatusCode ActivationGradient(const size_t m, const size_t n, const void* y_buffer, const size_t y_offset, const size_t y_ld,
+                              const Activation activation, const void* pre_buffer, const size_t pre_offset,
+                              const size_t pre_ld, void* c_buffer, const size_t c_offset, const size_t c_ld,
+                              void* bias_gradient_buffer, const size_t bias_gradient_offset, const size_t group_count,
+                              const void* group_offsets, const size_t group_offsets_offset, hipStream_t* queue,
+                              hipEvent_t* event = nullptr);
+
+// For every group g: Z = alpha * A_g * op(B_g) + bias_g, C_g = act(Z) + beta * C_g. The rows of A (m x k), C and pre (m x n)
+// belong to groups: group g owns the rows offsets[g] .. offsets[g + 1] - 1, offsets being group_count + 1 ascending 64-bit
+// integers in DEVICE memory (group_offsets, an element offset from there), so a router's counts need not come to the
+// host. A group may be empty. Rows in front of the first and behind the last group are neither read nor written. Matrix g
+// of B starts b_stride elements behind the one before (0: all groups share one), its bias bias_stride elements. Values that
+// do not ascend or lead outside 0 .. m are clamped so that no access leaves the matrices; what C holds then is not specified. m is
+// below 2^26.
+template <typename T>
+StatusCode GemmGrouped(const Transpose b_transpose, const size_t m, const size_t n, const size_t k, const float alpha,
+                       const void* a_buffer, const size_t a_offset, const size_t a_ld, const void* b_buffer,
+                       const size_t b_offset, const size_t b_ld, const size_t b_stride, const void* bias_buffer,
+                       const size_t bias_offset, const size_t bias_stride, const Activation activation, void* pre_buffer,
+                       const size_t pre_offset, const size_t pre_ld, const float beta, void* c_buffer, const size_t c_offset,
+                       const size_t c_ld, const size_t group_count, const void* group_offsets,
+                       const size_t group_offsets_offset, hipStream_t* queue, hipEvent_t* event = nullptr);
+
+// C_g = alpha * A_g^T * B_g + beta * C_g (m x n, c_stride elements apart) for every group g, A_g and B_g being the group's
+// rows of A (k x m) and B (k x n): the gradients of the groups' weights. A group without rows gives beta * C_g (zeros for
+// beta = 0). Groups as for GemmGrouped; k is below 2^26.
+template <typename T>
+StatusCode GemmGroupedGradient(const size_t m, const size_t n, const size_t k, const float alpha, const void* a_buffer,
+                               const size_t a_offset, const size_t a_ld, const void* b_buffer, const size_t b_offset,
+                               const size_t b_ld, const float beta, void* c_buffer, const size_t c_offset, const size_t c_ld,
+                               const size_t c_stride, const size_t group_count, const void* group_offsets,
+                               const size_t group_offsets_offset, hipStream_t* queue, hipEvent_t* event = nullptr);
 
 // Bytes this engine wants in `temp_buffer` for the given arguments (0 when none is needed). T as for Gemm.
 template <typename T>

@@ -40,13 +40,18 @@ typedef enum CLBlastStatusCode_ {
   CLBlastInvalidMatrixA = -1022,
   CLBlastInvalidMatrixB = -1021,
   CLBlastInvalidMatrixC = -1020,
+  CLBlastInvalidVectorX = -1019,
+  CLBlastInvalidVectorY = -1018,
   CLBlastInvalidDimension = -1017,
   CLBlastInvalidLeadDimA = -1016,
   CLBlastInvalidLeadDimB = -1015,
   CLBlastInvalidLeadDimC = -1014,
+  CLBlastInvalidIncrementX = -1013,
   CLBlastInsufficientMemoryA = -1011,
   CLBlastInsufficientMemoryB = -1010,
   CLBlastInsufficientMemoryC = -1009,
+  CLBlastInsufficientMemoryX = -1008,
+  CLBlastInsufficientMemoryY = -1007,
   CLBlastInsufficientMemoryTemp = -2050,
   CLBlastInvalidBatchCount = -2049,
   CLBlastInvalidOverrideKernel = -2048,
@@ -70,6 +75,13 @@ typedef struct CLBlastDouble2_ { double x; double y; } CLBlastDouble2;
 typedef enum CLBlastTriangle_ { CLBlastTriangleUpper = 121, CLBlastTriangleLower = 122 } CLBlastTriangle;
 typedef enum CLBlastDiagonal_ { CLBlastDiagonalNonUnit = 131, CLBlastDiagonalUnit = 132 } CLBlastDiagonal;
 typedef enum CLBlastKernelMode_ { CLBlastKernelModeCrossCorrelation = 151, CLBlastKernelModeConvolution = 152 } CLBlastKernelMode;
+typedef enum CLBlastActivation_ {  // see clblast::Activation
+  CLBlastActivationNone = 161,
+  CLBlastActivationRelu = 162,
+  CLBlastActivationGelu = 163,
+  CLBlastActivationGeluTanh = 164,
+  CLBlastActivationSilu = 165
+} CLBlastActivation;
 typedef enum CLBlastSide_ { CLBlastSideLeft = 141, CLBlastSideRight = 142 } CLBlastSide;
 typedef enum CLBlastPrecision_ {
   CLBlastPrecisionHalf = 16,
@@ -351,6 +363,101 @@ CLBlastStatusCode CLBLAST_HIP_API CLBlastHconvgemm(const CLBlastKernelMode kerne
                                                    const void* kernel_buffer, const size_t kernel_offset,
                                                    void* result_buffer, const size_t result_offset, hipStream_t* queue,
                                                    hipEvent_t* event);
+
+// =================================================================================================
+// Products of a network's layers (include/clblast_hip.h describes each; the reference has no such routines). All matrices
+// row-major; S: float, H: IEEE binary16, B: bfloat16 data; scalars are floats for all three. group_offsets: group_count + 1
+// ascending 64-bit integers in device memory.
+CLBlastStatusCode CLBLAST_HIP_API CLBlastSgemmEpilogue(const CLBlastTranspose a_transpose,
+    const CLBlastTranspose b_transpose, const size_t m, const size_t n, const size_t k, const float alpha, const void* a_buffer,
+    const size_t a_offset, const size_t a_ld, const void* b_buffer, const size_t b_offset, const size_t b_ld,
+    const void* bias_buffer, const size_t bias_offset, const CLBlastActivation activation, void* pre_buffer,
+    const size_t pre_offset, const size_t pre_ld, const float beta, const void* residual_buffer, const size_t residual_offset,
+    const size_t residual_ld, void* c_buffer, const size_t c_offset, const size_t c_ld, hipStream_t* queue,
+    hipEvent_t* event);
+CLBlastStatusCode CLBLAST_HIP_API CLBlastHgemmEpilogue(const CLBlastTranspose a_transpose,
+    const CLBlastTranspose b_transpose, const size_t m, const size_t n, const size_t k, const float alpha, const void* a_buffer,
+    const size_t a_offset, const size_t a_ld, const void* b_buffer, const size_t b_offset, const size_t b_ld,
+    const void* bias_buffer, const size_t bias_offset, const CLBlastActivation activation, void* pre_buffer,
+    const size_t pre_offset, const size_t pre_ld, const float beta, const void* residual_buffer, const size_t residual_offset,
+    const size_t residual_ld, void* c_buffer, const size_t c_offset, const size_t c_ld, hipStream_t* queue,
+    hipEvent_t* event);
+CLBlastStatusCode CLBLAST_HIP_API CLBlastBgemmEpilogue(const CLBlastTranspose a_transpose,
+    const CLBlastTranspose b_transpose, const size_t m, const size_t n, const size_t k, const float alpha, const void* a_buffer,
+    const size_t a_offset, const size_t a_ld, const void* b_buffer, const size_t b_offset, const size_t b_ld,
+    const void* bias_buffer, const size_t bias_offset, const CLBlastActivation activation, void* pre_buffer,
+    const size_t pre_offset, const size_t pre_ld, const float beta, const void* residual_buffer, const size_t residual_offset,
+    const size_t residual_ld, void* c_buffer, const size_t c_offset, const size_t c_ld, hipStream_t* queue,
+    hipEvent_t* event);
+CLBlastStatusCode CLBLAST_HIP_API CLBlastSgemmActivationGradient(const CLBlastTranspose a_transpose,
+    const CLBlastTranspose b_transpose, const size_t m, const size_t n, const size_t k, const float alpha,
+    const void* a_buffer, const size_t a_offset, const size_t a_ld, const void* b_buffer, const size_t b_offset, const size_t b_ld,
+    const CLBlastActivation activation, const void* pre_buffer, const size_t pre_offset, const size_t pre_ld,
+    void* c_buffer, const size_t c_offset, const size_t c_ld, void* bias_gradient_buffer, const size_t bias_gradient_offset,
+    hipStream_t* queue, hipEvent_t* event);
+CLBlastStatusCode CLBLAST_HIP_API CLBlastHgemmActivationGradient(const CLBlastTranspose a_transpose,
+    const CLBlastTranspose b_transpose, const size_t m, const size_t n, const size_t k, const float alpha,
+    const void* a_buffer, const size_t a_offset, const size_t a_ld, const void* b_buffer, const size_t b_offset, const size_t b_ld,
+    const CLBlastActivation activation, const void* pre_buffer, const size_t pre_offset, const size_t pre_ld,
+    void* c_buffer, const size_t c_offset, const size_t c_ld, void* bias_gradient_buffer, const size_t bias_gradient_offset,
+    hipStream_t* queue, hipEvent_t* event);
+CLBlastStatusCode CLBLAST_HIP_API CLBlastBgemmActivationGradient(const CLBlastTranspose a_transpose,
+    const CLBlastTranspose b_transpose, const size_t m, const size_t n, const size_t k, const float alpha,
+    const void* a_buffer, const size_t a_offset, const size_t a_ld, const void* b_buffer, const size_t b_offset, const size_t b_ld,
+    const CLBlastActivation activation, const void* pre_buffer, const size_t pre_offset, const size_t pre_ld,
+    void* c_buffer, const size_t c_offset, const size_t c_ld, void* bias_gradient_buffer, const size_t bias_gradient_offset,
+    hipStream_t* queue, hipEvent_t* event);
+CLBlastStatusCode CLBLAST_HIP_API CLBlastSactivationGradient(const size_t m, const size_t n, const void* y_buffer,
+    const size_t y_offset, const size_t y_ld, const CLBlastActivation activation, const void* pre_buffer,
+    const size_t pre_offset, const size_t pre_ld, void* c_buffer, const size_t c_offset, const size_t c_ld,
+    void* bias_gradient_buffer, const size_t bias_gradient_offset, const size_t group_count, const void* group_offsets,
+    const size_t group_offsets_offset, hipStream_t* queue, hipEvent_t* event);
+CLBlastStatusCode CLBLAST_HIP_API CLBlastHactivationGradient(const size_t m, const size_t n, const void* y_buffer,
+    const size_t y_offset, const size_t y_ld, const CLBlastActivation activation, const void* pre_buffer,
+    const size_t pre_offset, const size_t pre_ld, void* c_buffer, const size_t c_offset, const size_t c_ld,
+    void* bias_gradient_buffer, const size_t bias_gradient_offset, const size_t group_count, const void* group_offsets,
+    const size_t group_offsets_offset, hipStream_t* queue, hipEvent_t* event);
+CLBlastStatusCode CLBLAST_HIP_API CLBlastBactivationGradient(const size_t m, const size_t n, const void* y_buffer,
+    const size_t y_offset, const size_t y_ld, const CLBlastActivation activation, const void* pre_buffer,
+    const size_t pre_offset, const size_t pre_ld, void* c_buffer, const size_t c_offset, const size_t c_ld,
+    void* bias_gradient_buffer, const size_t bias_gradient_offset, const size_t group_count, const void* group_offsets,
+    const size_t group_offsets_offset, hipStream_t* queue, hipEvent_t* event);
+CLBlastStatusCode CLBLAST_HIP_API CLBlastSgemmGrouped(const CLBlastTranspose b_transpose, const size_t m,
+    const size_t n, const size_t k, const float alpha, const void* a_buffer, const size_t a_offset, const size_t a_ld,
+    const void* b_buffer, const size_t b_offset, const size_t b_ld, const size_t b_stride, const void* bias_buffer,
+    const size_t bias_offset, const size_t bias_stride, const CLBlastActivation activation, void* pre_buffer,
+    const size_t pre_offset, const size_t pre_ld, const float beta, void* c_buffer, const size_t c_offset, const size_t c_ld,
+    const size_t group_count, const void* group_offsets, const size_t group_offsets_offset, hipStream_t* queue,
+    hipEvent_t* event);
+CLBlastStatusCode CLBLAST_HIP_API CLBlastHgemmGrouped(const CLBlastTranspose b_transpose, const size_t m,
+    const size_t n, const size_t k, const float alpha, const void* a_buffer, const size_t a_offset, const size_t a_ld,
+    const void* b_buffer, const size_t b_offset, const size_t b_ld, const size_t b_stride, const void* bias_buffer,
+    const size_t bias_offset, const size_t bias_stride, const CLBlastActivation activation, void* pre_buffer,
+    const size_t pre_offset, const size_t pre_ld, const float beta, void* c_buffer, const size_t c_offset, const size_t c_ld,
+    const size_t group_count, const void* group_offsets, const size_t group_offsets_offset, hipStream_t* queue,
+    hipEvent_t* event);
+CLBlastStatusCode CLBLAST_HIP_API CLBlastBgemmGrouped(const CLBlastTranspose b_transpose, const size_t m,
+    const size_t n, const size_t k, const float alpha, const void* a_buffer, const size_t a_offset, const size_t a_ld,
+    const void* b_buffer, const size_t b_offset, const size_t b_ld, const size_t b_stride, const void* bias_buffer,
+    const size_t bias_offset, const size_t bias_stride, const CLBlastActivation activation, void* pre_buffer,
+    const size_t pre_offset, const size_t pre_ld, const float beta, void* c_buffer, const size_t c_offset, const size_t c_ld,
+    const size_t group_count, const void* group_offsets, const size_t group_offsets_offset, hipStream_t* queue,
+    hipEvent_t* event);
+CLBlastStatusCode CLBLAST_HIP_API CLBlastSgemmGroupedGradient(const size_t m, const size_t n, const size_t k,
+    const float alpha, const void* a_buffer, const size_t a_offset, const size_t a_ld, const void* b_buffer,
+    const size_t b_offset, const size_t b_ld, const float beta, void* c_buffer, const size_t c_offset, const size_t c_ld,
+    const size_t c_stride, const size_t group_count, const void* group_offsets, const size_t group_offsets_offset,
+    hipStream_t* queue, hipEvent_t* event);
+CLBlastStatusCode CLBLAST_HIP_API CLBlastHgemmGroupedGradient(const size_t m, const size_t n, const size_t k,
+    const float alpha, const void* a_buffer, const size_t a_offset, const size_t a_ld, const void* b_buffer,
+    const size_t b_offset, const size_t b_ld, const float beta, void* c_buffer, const size_t c_offset, const size_t c_ld,
+    const size_t c_stride, const size_t group_count, const void* group_offsets, const size_t group_offsets_offset,
+    hipStream_t* queue, hipEvent_t* event);
+CLBlastStatusCode CLBLAST_HIP_API CLBlastBgemmGroupedGradient(const size_t m, const size_t n, const size_t k,
+    const float alpha, const void* a_buffer, const size_t a_offset, const size_t a_ld, const void* b_buffer,
+    const size_t b_offset, const size_t b_ld, const float beta, void* c_buffer, const size_t c_offset, const size_t c_ld,
+    const size_t c_stride, const size_t group_count, const void* group_offsets, const size_t group_offsets_offset,
+    hipStream_t* queue, hipEvent_t* event);
 
 // Triangular solve in place: B becomes the X with op(A)*X = alpha*B (side left) or X*op(A) = alpha*B (side right)
 // replaces CLBlastStrsm/CLBlastDtrsm/CLBlastCtrsm/CLBlastZtrsm; like the reference there is no half-precision TRSM
