@@ -399,32 +399,40 @@ def gemmStridedBatched(queue, m, n, k, batch_count, a, b, c, a_ld, b_ld, c_ld, a
 # tensors are None. ``activation`` is one of ACTIVATIONS. The headers describe the operators (include/clblast_hip.h).
 
 _LAYER_PREFIX = {"torch.float32": "S", "torch.float16": "H", "torch.bfloat16": "B"}
+_layer_functions = {}  # (routine, dtype) -> the C function
+
+
+def _layer_function(routine, dtype):
+    prefix = _LAYER_PREFIX.get(str(dtype))
+    if prefix is None:
+        raise ValueError("PyCLBlast: unrecognized data-type '%s'" % dtype)
+    return _layer_functions.setdefault((routine, dtype), getattr(_lib.load(), "CLBlast%s%s" % (prefix, routine)))
 
 
 def _layer(routine, queue, tensors, group_offsets, arguments):
+    import torch
     first = tensors[0]
+    dtype, device = first.dtype, first.device
     for t in tensors:
         if t is not None:
-            if t.dtype != first.dtype:
-                raise ValueError("PyCLBlast: All arrays have to be of the same data-type, got: %s and %s" % (first.dtype, t.dtype))
-            if not t.is_cuda or t.device != first.device:
+            if t.dtype is not dtype:
+                raise ValueError("PyCLBlast: All arrays have to be of the same data-type, got: %s and %s" % (dtype, t.dtype))
+            if t.device != device:
                 raise ValueError("PyCLBlast: operands must live on one GPU")
+    if not first.is_cuda:
+        raise ValueError("PyCLBlast: operands must live on the GPU")
     if group_offsets is not None:
-        if str(group_offsets.dtype) != "torch.int64" or not group_offsets.is_contiguous():
+        if group_offsets.dtype is not torch.int64 or not group_offsets.is_contiguous():
             raise ValueError("PyCLBlast: group_offsets must be contiguous 64-bit integers")
-        if group_offsets.device != first.device:
+        if group_offsets.device != device:
             raise ValueError("PyCLBlast: operands must live on one GPU")
-    prefix = _LAYER_PREFIX.get(str(first.dtype))
-    if prefix is None:
-        raise ValueError("PyCLBlast: unrecognized data-type '%s'" % first.dtype)
-    if queue is None:  # (the stream's device must be the current one, and so must the operands')
-        import torch
-        if first.device.index != torch.cuda.current_device():
-            raise ValueError("PyCLBlast: operands must live on the current GPU")
-    function = getattr(_lib.load(), "CLBlast%s%s" % (prefix, routine))
-    status = function(*arguments, _stream_ref(_stream_handle(queue)), None)
+    stream = torch.cuda.current_stream() if queue is None else queue
+    if stream.device != device or device.index != torch.cuda.current_device():  # (the device of a launch is the current one)
+        raise ValueError("PyCLBlast: the operands' GPU must be the queue's and the current one")
+    function = _layer_functions.get((routine, dtype)) or _layer_function(routine, dtype)
+    status = function(*arguments, _stream_ref(stream.cuda_stream), None)
     if status != 0:
-        raise CLBlastError("CLBlast%s%s" % (prefix, routine), status)
+        raise CLBlastError("CLBlast%s%s" % (_LAYER_PREFIX[str(dtype)], routine), status)
 
 
 def _activation(name):

@@ -12,12 +12,6 @@ int Units() {
   return (clbh_compute_units(&units) == 0 && units > 0) ? units : 256;
 }
 
-bool OperandFits(const void* pointer, const long long ld, const long long stride, const int type) {
-  if (ld >= CLBH_LAYER_MAX_LD) { return false; }
-  if (type == CLBH_TYPE_FP32) { return true; }
-  return reinterpret_cast<unsigned long long>(pointer) % 4 == 0 && ld % 2 == 0 && stride % 2 == 0;
-}
-
 // Every access of the kernels follows from these: sizes, leading dimensions that hold a line, pointers where they are used
 bool ValidLayer(const clbh_layer_desc& d) {
   const auto aligned = [&](const void* pointer) {
@@ -29,7 +23,7 @@ bool ValidLayer(const clbh_layer_desc& d) {
     if (d.offsets == nullptr || reinterpret_cast<unsigned long long>(d.offsets) % 8 != 0 || d.groups <= 0 || d.groups > CLBH_LAYER_MAX_GROUPS) { return false; }
     if ((d.grouping == CLBH_GROUPS_BY_ROWS ? d.n : d.k) >= CLBH_LAYER_MAX_GROUPED) { return false; }
   }
-  if (!aligned(d.c) || !aligned(d.pre) || !aligned(d.residual) || !aligned(d.bias) || !aligned(d.upstream) || !aligned(d.bias_gradient)) { return false; }
+  if (!aligned(d.c) || !aligned(d.pre) || !aligned(d.residual) || !aligned(d.bias) || !aligned(d.upstream) || !aligned(d.bias_gradient) || !aligned(d.a) || !aligned(d.b)) { return false; }
   if (d.c != nullptr && d.c_ld < d.m) { return false; }
   if (d.pre != nullptr && d.pre_ld < d.m) { return false; }
   if (!d.gradient && d.beta != 0.0f && (d.residual == nullptr || d.residual_ld < d.m)) { return false; }
@@ -43,20 +37,12 @@ bool ValidLayer(const clbh_layer_desc& d) {
   if (d.a_ld < (d.a_kcontig ? d.k : d.m) || d.b_ld < (d.b_kcontig ? d.k : d.n)) { return false; }
   if (by_rows && (!d.b_kcontig || d.a_stride < 0 || d.bias_stride < 0 || d.gradient)) { return false; }
   if (by_depth && (d.a_kcontig || d.b_kcontig || d.c_stride < 0 || d.gradient || d.bias != nullptr || d.pre != nullptr || d.activation != 161)) { return false; }
-  if (by_depth && d.beta != 0.0f && d.residual != d.c) { return false; }
-  int copy = 0;
-  return clbh_layer_operands_fit(&d, &copy) != 0;
+  return !by_depth || d.beta == 0.0f || d.residual == d.c;
 }
 
 }  // namespace
 
 extern "C" {
-
-int clbh_layer_operands_fit(const clbh_layer_desc* desc, int* copy) {
-  const auto& d = *desc;
-  *copy = (OperandFits(d.a, d.a_ld, d.grouping == CLBH_GROUPS_BY_ROWS ? d.a_stride : 0, d.type) ? 0 : 1) | (OperandFits(d.b, d.b_ld, 0, d.type) ? 0 : 2);
-  return *copy == 0 ? 1 : 0;
-}
 
 size_t clbh_layer_workspace_bytes(const clbh_layer_desc* desc) {
   return (desc != nullptr && desc->m > 0 && desc->n > 0) ? PlanLayer(*desc, Units()).workspace_bytes : 0;

@@ -45,18 +45,12 @@ inline LayerArgs MakeLayerArgs(const clbh_layer_desc& d, const LayerPlan& plan) 
   p.grouping = d.grouping;
   p.groups = d.groups;
   p.offsets = d.offsets;
-  const long long size = (d.type == CLBH_TYPE_FP32) ? 4 : 2;
-  const auto movable = [&](const void* pointer, const long long ld) {
-    return pointer == nullptr || (reinterpret_cast<unsigned long long>(pointer) % 4 == 0 && (ld * size) % 4 == 0);
-  };
-  p.vector_rows = movable(d.c, d.c_ld) && movable(d.c, d.c_stride) && movable(d.pre, d.pre_ld) &&
-                  (d.beta == 0.0f || movable(d.residual, d.residual_ld)) && movable(d.upstream, d.upstream_ld);
   if (plan.splits > 1) {
     p.split_chunk = plan.chunk;
     p.partials = static_cast<float*>(d.workspace);
   }
   if (d.bias_gradient != nullptr) {
-    p.bias_partials = reinterpret_cast<float*>(static_cast<char*>(d.workspace) + plan.partial_bytes);
+    p.bias_partials = reinterpret_cast<float*>(static_cast<char*>(d.workspace) + plan.sums_offset);
   }
   return p;
 }
@@ -64,7 +58,8 @@ inline LayerArgs MakeLayerArgs(const clbh_layer_desc& d, const LayerPlan& plan) 
 template <typename Config, bool A_KC, bool B_KC>
 int LaunchLayerTile(const clbh_layer_desc& d, const LayerPlan& plan, const LayerArgs& args, hipStream_t stream) {
   if (Config::TILE_M != plan.tile.tile_m || Config::TILE_N != plan.tile.tile_n) { return hipErrorInvalidValue; }
-  const long long blocks = plan.tiles_m * plan.tiles_n * ((d.grouping == CLBH_GROUPS_BY_DEPTH) ? d.groups : 1);
+  // (groups by depth: every XCD takes an eighth of each group's tiles)
+  const long long blocks = (d.grouping == CLBH_GROUPS_BY_DEPTH) ? d.groups * ((plan.tiles_m * plan.tiles_n + 7) / 8 * 8) : plan.tiles_m * plan.tiles_n;
   if (blocks > INT_MAX) { return hipErrorInvalidConfiguration; }
   auto kernel = LayerGemmKernel<Config, A_KC, B_KC>;
   constexpr int lds_bytes = Config::LDS_BYTES;
@@ -101,7 +96,7 @@ int LaunchLayerProduct(const clbh_layer_desc& d, const LayerPlan& plan, const La
   }
 }
 
-template <typename T, int V>
+template <typename T, int V, bool UPSTREAM>
 int LaunchLayerRowsOf(const clbh_layer_desc& d, const LayerPlan& plan, const LayerArgs& args, hipStream_t stream) {
   LayerRowsArgs q{};
   q.layer = args;
@@ -112,21 +107,62 @@ int LaunchLayerRowsOf(const clbh_layer_desc& d, const LayerPlan& plan, const Lay
   const long long column_blocks = (static_cast<long long>(d.m) + 64 * V - 1) / (64 * V);
   if (column_blocks * plan.rows_chunks > INT_MAX) { return hipErrorInvalidConfiguration; }
   q.column_blocks = static_cast<int>(column_blocks);
-  LayerRowsKernel<T, V><<<dim3(static_cast<unsigned>(column_blocks * plan.rows_chunks)), dim3(kLayerRowsThreads), 0, stream>>>(q);
+  LayerRowsKernel<T, V, UPSTREAM><<<dim3(static_cast<unsigned>(column_blocks * plan.rows_chunks)), dim3(kLayerRowsThreads), 0, stream>>>(q);
+  return static_cast<int>(hipGetLastError());
+}
+
+// Copies the operands that do not fit (LayerOperandFits) into the workspace, in one launch, and puts the copies in their place
+template <typename T>
+int AlignLayerOperands(const clbh_layer_desc& d, const LayerPlan& plan, LayerArgs& args, hipStream_t stream) {
+  LayerAlignArgs q{};
+  long long blocks[2] = {0, 0};
+  const auto describe = [&](const int index, const void* from, const long long ld, const long long stride, const long long new_ld,
+                            const size_t offset, const int length, const int lines, const int matrices) {
+    auto& o = q.operand[index];
+    o.from = from;
+    o.to = static_cast<char*>(d.workspace) + offset;
+    o.ld = ld;
+    o.stride = stride;
+    o.new_ld = new_ld;
+    o.length = length;
+    o.lines = lines;
+    o.matrices = matrices;
+    while (o.lane_shift < 6 && (16ll / static_cast<long long>(sizeof(T)) << o.lane_shift) < length) { ++o.lane_shift; }
+    const long long lines_per_block = kLayerRowsThreads >> o.lane_shift;
+    blocks[index] = (static_cast<long long>(lines) * matrices + lines_per_block - 1) / lines_per_block;
+  };
+  const bool by_rows = d.grouping == CLBH_GROUPS_BY_ROWS;
+  if (plan.a_copy_ld > 0) {
+    const int lines = d.a_kcontig ? d.m : d.k;
+    describe(0, d.a, d.a_ld, by_rows ? d.a_stride : 0, plan.a_copy_ld, plan.a_copy_offset, d.a_kcontig ? d.k : d.m, lines, by_rows ? d.groups : 1);
+    args.a = q.operand[0].to;
+    args.a_ld = plan.a_copy_ld;
+    args.a_stride = plan.a_copy_ld * lines;
+  }
+  if (plan.b_copy_ld > 0) {
+    describe(1, d.b, d.b_ld, 0, plan.b_copy_ld, plan.b_copy_offset, d.b_kcontig ? d.k : d.n, d.b_kcontig ? d.n : d.k, 1);
+    args.b = q.operand[1].to;
+    args.b_ld = plan.b_copy_ld;
+  }
+  if (blocks[0] + blocks[1] == 0) { return 0; }
+  if (blocks[0] + blocks[1] > INT_MAX) { return hipErrorInvalidConfiguration; }
+  q.blocks_of_first = static_cast<int>(blocks[0]);
+  LayerAlignKernel<T><<<dim3(static_cast<unsigned>(blocks[0] + blocks[1])), dim3(kLayerRowsThreads), 0, stream>>>(q);
   return static_cast<int>(hipGetLastError());
 }
 
 template <typename T>
 int LaunchLayerTyped(const clbh_layer_desc& d, const LayerPlan& plan, hipStream_t stream) {
-  const auto args = MakeLayerArgs(d, plan);
+  auto args = MakeLayerArgs(d, plan);
   const bool elementwise = d.upstream != nullptr || plan.splits > 1;
   if (d.upstream == nullptr) {
-    const int status = LaunchLayerProduct<T>(d, plan, args, stream);
+    int status = AlignLayerOperands<T>(d, plan, args, stream);
+    if (status == 0) { status = LaunchLayerProduct<T>(d, plan, args, stream); }
     if (status != 0) { return status; }
   }
   if (elementwise) {
-    constexpr int V = 16 / sizeof(T);
-    const int status = args.vector_rows ? LaunchLayerRowsOf<T, V>(d, plan, args, stream) : LaunchLayerRowsOf<T, 1>(d, plan, args, stream);
+    // (of the fp32 sums of K ranges a lane takes four, 16 bytes)
+    const int status = (d.upstream != nullptr) ? LaunchLayerRowsOf<T, 16 / sizeof(T), true>(d, plan, args, stream) : LaunchLayerRowsOf<T, 4, false>(d, plan, args, stream);
     if (status != 0) { return status; }
   }
   if (d.bias_gradient != nullptr) {

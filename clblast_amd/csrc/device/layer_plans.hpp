@@ -29,8 +29,18 @@ struct LayerPlan {
   int splits, chunk;           // K ranges (1: none)
   int rows_chunk;              // rows per work-group of the elementwise kernel
   long long rows_chunks;       // work-groups of it along the rows (the most there can be)
-  size_t partial_bytes, sums_bytes, workspace_bytes;
+  // operands that the kernel cannot fetch as they are and that are copied first (0: not), with the copy's leading dimension
+  long long a_copy_ld, b_copy_ld;
+  // the workspace: sums of K ranges, sums for the bias gradient, copies of a and b
+  size_t sums_offset, a_copy_offset, b_copy_offset, workspace_bytes;
 };
+
+// 16-bit operands are fetched in dwords: their lines (and the groups' matrices) have to start at dwords. The lines of a slab
+// are reached by 32-bit byte offsets.
+inline bool LayerOperandFits(const void* pointer, const long long ld, const long long stride, const int type) {
+  if (ld >= CLBH_LAYER_MAX_LD) { return false; }
+  return type == CLBH_TYPE_FP32 || (reinterpret_cast<unsigned long long>(pointer) % 4 == 0 && ld % 2 == 0 && stride % 2 == 0);
+}
 
 // Most tiles of `tile` rows that `groups` ranges within `rows` rows can be cut into: every group can add one that is not full
 inline long long MostGroupTiles(const long long rows, const long long groups, const long long tile) {
@@ -54,6 +64,11 @@ inline int LayerVector(const int type) { return type == CLBH_TYPE_FP32 ? 4 : 8; 
 inline LayerPlan PlanLayer(const clbh_layer_desc& d, const int units) {
   auto plan = LayerPlan{};
   plan.splits = 1;
+  const auto take = [&](const size_t bytes) {  // a piece of the workspace
+    const size_t offset = plan.workspace_bytes;
+    plan.workspace_bytes += (bytes + 255) / 256 * 256;
+    return offset;
+  };
   if (d.upstream == nullptr) {
     const auto count = [&](const LayerTile& t) {
       const long long along_m = (d.m + t.tile_m - 1) / t.tile_m;
@@ -79,19 +94,29 @@ inline LayerPlan PlanLayer(const clbh_layer_desc& d, const int units) {
       if (splits > 1 && splits <= 65535) {
         plan.splits = splits;
         plan.chunk = chunk;
-        plan.partial_bytes = sizeof(float) * static_cast<size_t>(splits) * static_cast<size_t>(d.n) * static_cast<size_t>(d.m);
-        plan.partial_bytes = (plan.partial_bytes + 255) / 256 * 256;
+        take(sizeof(float) * static_cast<size_t>(splits) * static_cast<size_t>(d.n) * static_cast<size_t>(d.m));
       }
     }
   }
-  const long long column_blocks = (d.m + 64ll * LayerVector(d.type) - 1) / (64ll * LayerVector(d.type));
+  const long long per_block = 64ll * ((d.upstream != nullptr) ? LayerVector(d.type) : 4), column_blocks = (d.m + per_block - 1) / per_block;
   plan.rows_chunk = LayerRowsChunk(d.n, column_blocks);
   plan.rows_chunks = (d.grouping == CLBH_GROUPS_BY_ROWS) ? MostGroupTiles(d.n, d.groups, plan.rows_chunk) : (d.n + plan.rows_chunk - 1) / plan.rows_chunk;
   if (d.bias_gradient != nullptr) {
     const long long rows_of_sums = (d.upstream != nullptr || plan.splits > 1) ? plan.rows_chunks : plan.tiles_n;
-    plan.sums_bytes = sizeof(float) * static_cast<size_t>(rows_of_sums) * static_cast<size_t>(d.m);
+    plan.sums_offset = take(sizeof(float) * static_cast<size_t>(rows_of_sums) * static_cast<size_t>(d.m));
   }
-  plan.workspace_bytes = plan.partial_bytes + plan.sums_bytes;
+  if (d.upstream == nullptr) {
+    const size_t size = (d.type == CLBH_TYPE_FP32) ? 4 : 2;
+    const bool by_rows = d.grouping == CLBH_GROUPS_BY_ROWS;
+    if (!LayerOperandFits(d.a, d.a_ld, by_rows ? d.a_stride : 0, d.type)) {
+      plan.a_copy_ld = ((d.a_kcontig ? d.k : d.m) + 7ll) / 8 * 8;
+      plan.a_copy_offset = take(size * static_cast<size_t>(plan.a_copy_ld) * static_cast<size_t>(d.a_kcontig ? d.m : d.k) * static_cast<size_t>(by_rows ? d.groups : 1));
+    }
+    if (!LayerOperandFits(d.b, d.b_ld, 0, d.type)) {
+      plan.b_copy_ld = ((d.b_kcontig ? d.k : d.n) + 7ll) / 8 * 8;
+      plan.b_copy_offset = take(size * static_cast<size_t>(plan.b_copy_ld) * static_cast<size_t>(d.b_kcontig ? d.n : d.k));
+    }
+  }
   return plan;
 }
 

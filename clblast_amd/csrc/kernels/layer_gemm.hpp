@@ -57,7 +57,6 @@ struct LayerArgs {
   int grouping;  // kLayerPlain, ...
   int groups;
   const long long* offsets;  // groups + 1 values
-  int vector_rows;           // C, pre, residual and bias can be moved in 16-byte pieces (dword-aligned rows)
   float* bias_partials;      // [tile of rows][m], or nullptr
   // K ranges of one plain product: range s goes to partials + s * n * m as fp32 sums, a second kernel finishes
   int split_chunk;
@@ -126,6 +125,25 @@ __device__ __forceinline__ bool FindGroupTile(const long long* __restrict__ offs
     passed += here;
   }
   return false;
+}
+
+// The group with the rank-th largest range, for up to 64 groups (one per lane; of equal ones the first comes first); rank itself
+// beyond
+__device__ __forceinline__ int GroupOfRank(const long long* __restrict__ offsets, const int groups, const int rows, const int rank,
+                                           const int lane) {
+  if (groups > 64) { return rank; }
+  int count = -1;
+  if (lane < groups) {
+    const long long from = offsets[lane], to = offsets[lane + 1];
+    const int first = static_cast<int>(from < 0 ? 0 : (from > rows ? rows : from));
+    count = static_cast<int>(to < first ? 0 : (to > rows ? rows : to) - first);
+  }
+  int above = 0;
+  for (int g = 0; g < groups; ++g) {
+    const int other = __builtin_amdgcn_readlane(count, g);
+    above += (other > count || (other == count && g < lane)) ? 1 : 0;
+  }
+  return __builtin_ctzll(__ballot(lane < groups && above == rank));
 }
 
 // ---- types and configurations ------------------------------------------------------------------------------------------
@@ -309,18 +327,16 @@ __device__ __forceinline__ void LayerValues(const LayerArgs& p, const float (&z)
   }
 }
 
-// V consecutive values of a row, of which the first `inside` exist; WHOLE: all of them do
+// V consecutive values of a row, of which the first `inside` exist, as one access at whatever address the row starts (the
+// hardware splits one that is not aligned)
 template <typename T, int V>
 struct LayerPiece {
-  typedef T Piece __attribute__((ext_vector_type(V), aligned(V == 1 ? sizeof(T) : 4)));
+  typedef T Piece __attribute__((ext_vector_type(V), aligned(sizeof(T))));
   static __device__ __forceinline__ void Load(const T* from, const int inside, float (&values)[V]) {
     if (inside >= V) {
-      if constexpr (V == 1) { values[0] = static_cast<float>(*from); }
-      else {
-        const Piece piece = *reinterpret_cast<const Piece*>(from);
+      const Piece piece = *reinterpret_cast<const Piece*>(from);
 #pragma unroll
-        for (int e = 0; e < V; ++e) { const T value = piece[e]; values[e] = static_cast<float>(value); }
-      }
+      for (int e = 0; e < V; ++e) { const T value = piece[e]; values[e] = static_cast<float>(value); }
     } else {
 #pragma unroll
       for (int e = 0; e < V; ++e) { values[e] = (e < inside) ? static_cast<float>(from[e]) : 0.0f; }
@@ -328,13 +344,10 @@ struct LayerPiece {
   }
   static __device__ __forceinline__ void Store(T* to, const int inside, const float (&values)[V]) {
     if (inside >= V) {
-      if constexpr (V == 1) { *to = static_cast<T>(values[0]); }
-      else {
-        Piece piece;
+      Piece piece;
 #pragma unroll
-        for (int e = 0; e < V; ++e) { piece[e] = static_cast<T>(values[e]); }
-        *reinterpret_cast<Piece*>(to) = piece;
-      }
+      for (int e = 0; e < V; ++e) { piece[e] = static_cast<T>(values[e]); }
+      *reinterpret_cast<Piece*>(to) = piece;
     } else {
 #pragma unroll
       for (int e = 0; e < V; ++e) { if (e < inside) { to[e] = static_cast<T>(values[e]); } }
@@ -344,28 +357,26 @@ struct LayerPiece {
 
 // Moves staged rows of a wavefront through the epilogue, lanes along the features in pieces of V values. The loop over
 // the rows is not unrolled (its body holds every activation); what it reads from memory is asked for two passes ahead.
-template <typename Config, int V>
+template <typename Config>
 struct LayerRows {
   using T = typename Config::T;
+  static constexpr int V = Config::VEC;
   using Piece = LayerPiece<T, V>;
   static constexpr bool FAST = sizeof(T) == 2;
-  static constexpr int PIECES = Config::WAVE_M / V;                    // of a row
-  static constexpr int ROW_LANES = PIECES < 64 ? PIECES : 64;
-  static constexpr int SETS = PIECES / ROW_LANES;                      // pieces of a row per lane
-  static constexpr int ROWS = 64 / ROW_LANES;                          // rows per pass
+  static constexpr int ROW_LANES = Config::WAVE_M / V;  // pieces of a row, one per lane
+  static constexpr int ROWS = 64 / ROW_LANES;           // rows per pass
   static constexpr int PASSES = Config::HALF_N / ROWS;
-  float bias[SETS][V], sums[SETS][V];
+  static_assert(ROW_LANES <= 64, "a row is at most one piece per lane");
+  float bias[V], sums[V];
 
   __device__ __forceinline__ void Begin(const T* bias_from, const int lane, const int inside) {
+    const int col = V * (lane % ROW_LANES);
 #pragma unroll
-    for (int set = 0; set < SETS; ++set) {
-      const int col = V * (lane % ROW_LANES + set * ROW_LANES);
-#pragma unroll
-      for (int e = 0; e < V; ++e) {
-        sums[set][e] = 0.0f;
-        bias[set][e] = (bias_from != nullptr && col + e < inside) ? static_cast<float>(bias_from[col + e]) : 0.0f;
-      }
+    for (int e = 0; e < V; ++e) {
+      sums[e] = 0.0f;
+      bias[e] = 0.0f;
     }
+    if (bias_from != nullptr) { Piece::Load(bias_from + col, inside - col, bias); }
   }
 
   // stage: the wavefront's staging tile of HALF_N rows, of which `rows` exist, each with `inside` features; c, pre, other: at
@@ -373,49 +384,41 @@ struct LayerRows {
   __device__ __forceinline__ void Run(const LayerArgs& p, const float* stage, T* c, T* pre, const T* other, const long long other_ld,
                                       const int lane, const int rows, const int inside) {
     constexpr int AHEAD = PASSES < 2 ? PASSES : 2;
+    const int row0 = lane / ROW_LANES, col = V * (lane % ROW_LANES);
+    const auto inside_of = [&](const int row) { return (row < rows) ? inside - col : 0; };
+    float old[AHEAD][V];
 #pragma unroll
-    for (int set = 0; set < SETS; ++set) {
-      const int row0 = lane / ROW_LANES, col = V * (lane % ROW_LANES + set * ROW_LANES);
-      const auto inside_of = [&](const int row) { return (row < rows) ? inside - col : 0; };
-      float old[AHEAD][V];
+    for (int u = 0; u < AHEAD; ++u) {
+#pragma unroll
+      for (int e = 0; e < V; ++e) { old[u][e] = 0.0f; }
+      const int row = row0 + u * ROWS;
+      if (other != nullptr) { Piece::Load(other + row * other_ld + col, inside_of(row), old[u]); }
+    }
+#pragma unroll 1
+    for (int pass = 0; pass < PASSES; pass += AHEAD) {
 #pragma unroll
       for (int u = 0; u < AHEAD; ++u) {
+        const int row = row0 + (pass + u) * ROWS;
+        float now[V], z[V], y[V];
 #pragma unroll
-        for (int e = 0; e < V; ++e) { old[u][e] = 0.0f; }
-        const int row = row0 + u * ROWS;
-        if (other != nullptr) { Piece::Load(other + row * other_ld + col, inside_of(row), old[u]); }
-      }
-#pragma unroll 1
-      for (int pass = 0; pass < PASSES; pass += AHEAD) {
+        for (int e = 0; e < V; ++e) { now[e] = old[u][e]; }
+        const int next = row + AHEAD * ROWS;
+        if (other != nullptr) { Piece::Load(other + next * other_ld + col, pass + u + AHEAD < PASSES ? inside_of(next) : 0, old[u]); }
+        const float* from = stage + row * Config::PITCH + col;
 #pragma unroll
-        for (int u = 0; u < AHEAD; ++u) {
-          const int row = row0 + (pass + u) * ROWS;
-          float now[V], z[V], y[V];
+        for (int q = 0; q < V; q += 4) {
+          const layer_float4_t four = *reinterpret_cast<const layer_float4_t*>(from + q);
 #pragma unroll
-          for (int e = 0; e < V; ++e) { now[e] = old[u][e]; }
-          const int next = row + AHEAD * ROWS;
-          if (other != nullptr) { Piece::Load(other + next * other_ld + col, pass + u + AHEAD < PASSES ? inside_of(next) : 0, old[u]); }
-          const float* from = stage + row * Config::PITCH + col;
-          if constexpr (V == 1) { z[0] = *from; }
-          else {
-#pragma unroll
-            for (int q = 0; q < V; q += 4) {
-              const layer_float4_t four = *reinterpret_cast<const layer_float4_t*>(from + q);
-#pragma unroll
-              for (int e = 0; e < 4; ++e) { z[q + e] = four[e]; }
-            }
-          }
-#pragma unroll
-          for (int e = 0; e < V; ++e) { z[e] = __builtin_fmaf(p.alpha, z[e], bias[set][e]); }
-          LayerValues<FAST>(p, z, now, y);
-          const int here = inside_of(row);
-          if (here > 0) {
-#pragma unroll
-            for (int e = 0; e < V; ++e) { sums[set][e] += y[e]; }
-          }
-          Piece::Store(c + row * p.c_ld + col, here, y);
-          if (pre != nullptr && !p.gradient) { Piece::Store(pre + row * p.pre_ld + col, here, z); }
+          for (int e = 0; e < 4; ++e) { z[q + e] = __builtin_fmaf(p.alpha, four[e], bias[q + e]); }
         }
+        LayerValues<FAST>(p, z, now, y);
+        const int here = inside_of(row);
+        if (here > 0) {
+#pragma unroll
+          for (int e = 0; e < V; ++e) { sums[e] += y[e]; }
+        }
+        Piece::Store(c + row * p.c_ld + col, here, y);
+        if (pre != nullptr && !p.gradient) { Piece::Store(pre + row * p.pre_ld + col, here, z); }
       }
     }
   }
@@ -423,14 +426,11 @@ struct LayerRows {
   // The wavefront's sums over its rows to `to` (LDS, WAVE_M values): lanes with the same features are added up first
   __device__ __forceinline__ void StoreSums(float* to, const int lane) {
 #pragma unroll
-    for (int set = 0; set < SETS; ++set) {
+    for (int e = 0; e < V; ++e) {
+      float sum = sums[e];
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        float sum = sums[set][e];
-#pragma unroll
-        for (int step = ROW_LANES; step < 64; step *= 2) { sum += __shfl_xor(sum, step, 64); }
-        if (lane < ROW_LANES) { to[V * (lane + set * ROW_LANES) + e] = sum; }
-      }
+      for (int step = ROW_LANES; step < 64; step *= 2) { sum += __shfl_xor(sum, step, 64); }
+      if (lane < ROW_LANES) { to[V * lane + e] = sum; }
     }
   }
 };
@@ -480,13 +480,15 @@ __global__ __launch_bounds__(Config::THREADS, Config::MIN_WAVES) void LayerGemmK
     tile_n = (local - walk * 8 * group_tiles) / height;
     sums_row = before + tile_n;
   } else if (p.grouping == kLayerGroupedDepth) {
-    const int index = XcdContiguousIndex(blockIdx.x, gridDim.x);
-    const int per_group = tiles_m * tiles_n;
-    group = index / per_group;
+    // The depths differ from group to group: every XCD (work-groups are dealt to the eight in turn) takes an eighth of every
+    // group's tiles, a contiguous one, and the groups come in the order of their depths, the deepest first.
+    const int share = (tiles_m * tiles_n + kNumXcd - 1) / kNumXcd;
+    const int local = static_cast<int>(blockIdx.x / kNumXcd) % share + static_cast<int>(blockIdx.x % kNumXcd) * share;
+    if (local >= tiles_m * tiles_n) { return; }
+    group = GroupOfRank(p.offsets, p.groups, p.k, blockIdx.x / kNumXcd / share, lane);
     int end;
     GroupRange(p.offsets, group, p.k, first, end);
     depth = end - first;
-    const int local = index - group * per_group;
     const int walk = local / (8 * tiles_n), height = min(tiles_m - 8 * walk, 8);
     tile_m = 8 * walk + (local - walk * 8 * tiles_n) % height;
     tile_n = (local - walk * 8 * tiles_n) / height;
@@ -727,38 +729,35 @@ __global__ __launch_bounds__(Config::THREADS, Config::MIN_WAVES) void LayerGemmK
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
   };
-  const auto finish = [&](auto rows_of) {
-    if (inside > 0) {
-      rows_of.Begin(bias, late_lane, inside);
+  if (inside > 0) {
+    LayerRows<Config> rows_of;
+    rows_of.Begin(bias, late_lane, inside);
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
+    for (int half = 0; half < 2; ++half) {
 #pragma unroll
-        for (int j = 0; j < HN; ++j) {
+      for (int j = 0; j < HN; ++j) {
 #pragma unroll
-          for (int i = 0; i < BM; ++i) {
+        for (int i = 0; i < BM; ++i) {
 #pragma unroll
-            for (int r = 0; r < static_cast<int>(sizeof(Acc) / 16); ++r) {
-              const int col = i * BLOCK + (BLOCK == 32 ? 8 * r + 4 * (late_lane / 32) : 4 * (late_lane / 16));
-              layer_float4_t run;
+          for (int r = 0; r < static_cast<int>(sizeof(Acc) / 16); ++r) {
+            const int col = i * BLOCK + (BLOCK == 32 ? 8 * r + 4 * (late_lane / 32) : 4 * (late_lane / 16));
+            layer_float4_t run;
 #pragma unroll
-              for (int e = 0; e < 4; ++e) { run[e] = acc[i][half * HN + j][4 * r + e]; }
-              *reinterpret_cast<layer_float4_t*>(&stage[(j * BLOCK + late_lane % BLOCK) * Config::PITCH + col]) = run;
-            }
+            for (int e = 0; e < 4; ++e) { run[e] = acc[i][half * HN + j][4 * r + e]; }
+            *reinterpret_cast<layer_float4_t*>(&stage[(j * BLOCK + late_lane % BLOCK) * Config::PITCH + col]) = run;
           }
         }
-        wave_fence();
-        const int n_block = n0 + wave_n * Config::WAVE_N + half * Config::HALF_N;
-        if (n_block < rows) {
-          rows_of.Run(p, stage, c + n_block * p.c_ld, (pre == nullptr) ? nullptr : pre + n_block * p.pre_ld,
-                      (other == nullptr) ? nullptr : other + n_block * other_ld, other_ld, late_lane, rows - n_block, inside);
-        }
-        wave_fence();
       }
-      if (p.bias_partials != nullptr) { rows_of.StoreSums(tile_sums + wave_n * TILE_M + wave_m * Config::WAVE_M, late_lane); }
+      wave_fence();
+      const int n_block = n0 + wave_n * Config::WAVE_N + half * Config::HALF_N;
+      if (n_block < rows) {
+        rows_of.Run(p, stage, c + n_block * p.c_ld, (pre == nullptr) ? nullptr : pre + n_block * p.pre_ld,
+                    (other == nullptr) ? nullptr : other + n_block * other_ld, other_ld, late_lane, rows - n_block, inside);
+      }
+      wave_fence();
     }
-  };
-  if (p.vector_rows) { finish(LayerRows<Config, Config::VEC>{}); }
-  else { finish(LayerRows<Config, 1>{}); }
+    if (p.bias_partials != nullptr) { rows_of.StoreSums(tile_sums + wave_n * TILE_M + wave_m * Config::WAVE_M, late_lane); }
+  }
   if (p.bias_partials != nullptr) {
     __syncthreads();
     for (int i = tid; i < TILE_M && m0 + i < p.m; i += Config::THREADS) {

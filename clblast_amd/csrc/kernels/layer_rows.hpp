@@ -3,6 +3,7 @@
 //   * LayerRowsKernel: the epilogue of kernels/layer_gemm.hpp on sums that are already there - the fp32 sums of a product
 //     whose K range was split over several work-groups (added up here in the order of the ranges), or, for the gradient of
 //     an activation, a matrix of the caller's. One pass over memory; bound by it.
+//   * LayerAlignKernel: copies of operands whose lines do not start at dwords, for the tiled kernel's loads.
 //   * LayerColumnSumsKernel: the second half of a bias gradient, which adds up the sums that the work-groups of either
 //     kernel left for their tiles of rows, in the order of the tiles: the result does not depend on timing.
 // =================================================================================================
@@ -24,20 +25,20 @@ struct LayerRowsArgs {
   int column_blocks;     // work-groups side by side; the grid's only dimension counts them first
 };
 
-// Work-group: 64 pieces of V features (lanes) times `chunk` rows, which its four wavefronts take in turn; four rows of a
-// wavefront are in flight at a time. bias_partials: one row of m sums for every chunk, the chunks numbered through the groups.
-template <typename T, int V>
-__global__ __launch_bounds__(kLayerRowsThreads) void LayerRowsKernel(const LayerRowsArgs q) {
+// Work-group: 64 pieces of V features (lanes) times `chunk` rows, which its four wavefronts take in turn. bias_partials: one
+// row of m sums for every chunk, the chunks numbered through the groups. UPSTREAM: the caller's matrix takes the place
+// of the sums.
+template <typename T, int V, bool UPSTREAM>
+__global__ __launch_bounds__(kLayerRowsThreads, UPSTREAM ? 5 : 4) void LayerRowsKernel(const LayerRowsArgs q) {
   constexpr bool FAST = sizeof(T) == 2;
-  constexpr int WAVES = kLayerRowsThreads / 64, FLIGHT = 4;
-  typedef float Four __attribute__((ext_vector_type(4), aligned(4)));
+  constexpr int WAVES = kLayerRowsThreads / 64, FLIGHT = UPSTREAM ? 2 : 1;  // rows of a wavefront in flight together
+  constexpr int RANGES = 8;                                                // K ranges in flight together
   const LayerArgs& p = q.layer;
   __shared__ float wave_sums[WAVES][64 * V];
   const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const int column_block = blockIdx.x % q.column_blocks;
   const int col = (column_block * 64 + lane) * V;
   const int inside = p.m - col;  // features from this lane's first one on
-  const bool whole = inside >= V;
 
   const int sums_row = blockIdx.x / q.column_blocks;
   int first, end;
@@ -55,52 +56,38 @@ __global__ __launch_bounds__(kLayerRowsThreads) void LayerRowsKernel(const Layer
 #pragma unroll
   for (int e = 0; e < V; ++e) {
     sums[e] = 0.0f;
-    bias[e] = (p.bias != nullptr && e < inside) ? static_cast<float>(static_cast<const T*>(p.bias)[col + e]) : 0.0f;
+    bias[e] = (!UPSTREAM && p.bias != nullptr && e < inside) ? static_cast<float>(static_cast<const T*>(p.bias)[col + e]) : 0.0f;
   }
   const T* other = p.gradient ? static_cast<const T*>(p.pre) : ((p.beta != 0.0f) ? static_cast<const T*>(p.residual) : nullptr);
   const long long other_ld = p.gradient ? p.pre_ld : p.residual_ld;
-  const auto load_sums = [&](const float* from, float* values) {
-    if (whole) {
-      if constexpr (V == 1) { values[0] = *from; }
-      else {
-#pragma unroll
-        for (int h = 0; h < V; h += 4) {
-          const Four four = *reinterpret_cast<const Four*>(from + h);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) { values[h + e] = four[e]; }
-        }
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < V; ++e) { values[e] = (e < inside) ? from[e] : 0.0f; }
-    }
-  };
+
   if (inside > 0) {
     for (int row0 = first + wave; row0 < end; row0 += WAVES * FLIGHT) {
       float z[FLIGHT][V], old[FLIGHT][V];
 #pragma unroll
       for (int u = 0; u < FLIGHT; ++u) {
         const long long row = min(row0 + WAVES * u, end - 1);  // (a row beyond the chunk: the last one again, not used)
-        if (q.upstream != nullptr) { LayerPiece<T, V>::Load(static_cast<const T*>(q.upstream) + row * q.upstream_ld + col, inside, z[u]); }
-        else { load_sums(p.partials + row * p.m + col, z[u]); }
+#pragma unroll
+        for (int e = 0; e < V; ++e) { z[u][e] = 0.0f; old[u][e] = 0.0f; }
+        if constexpr (UPSTREAM) { LayerPiece<T, V>::Load(static_cast<const T*>(q.upstream) + row * q.upstream_ld + col, inside, z[u]); }
         if (other != nullptr) { LayerPiece<T, V>::Load(other + row * other_ld + col, inside, old[u]); }
-        else {
-#pragma unroll
-          for (int e = 0; e < V; ++e) { old[u][e] = 0.0f; }
-        }
       }
-      for (int range = 1; range < q.ranges; ++range) {
-        const float* slab = p.partials + static_cast<long long>(range) * p.n * p.m;
-        float more[FLIGHT][V];
+      if constexpr (!UPSTREAM) {
+        const float* from = p.partials + static_cast<long long>(row0) * p.m + col;
+        const long long slab = static_cast<long long>(p.n) * p.m;
+        for (int range = 0; range < q.ranges; range += RANGES) {
+          float more[RANGES][V];
 #pragma unroll
-        for (int u = 0; u < FLIGHT; ++u) {
-          const long long row = min(row0 + WAVES * u, end - 1);
-          load_sums(slab + row * p.m + col, more[u]);
-        }
+          for (int r = 0; r < RANGES; ++r) {
 #pragma unroll
-        for (int u = 0; u < FLIGHT; ++u) {
+            for (int e = 0; e < V; ++e) { more[r][e] = 0.0f; }
+            if (range + r < q.ranges) { LayerPiece<float, V>::Load(from + (range + r) * slab, inside, more[r]); }
+          }
 #pragma unroll
-          for (int e = 0; e < V; ++e) { z[u][e] += more[u][e]; }
+          for (int r = 0; r < RANGES; ++r) {
+#pragma unroll
+            for (int e = 0; e < V; ++e) { z[0][e] += more[r][e]; }
+          }
         }
       }
 #pragma unroll
@@ -108,13 +95,15 @@ __global__ __launch_bounds__(kLayerRowsThreads) void LayerRowsKernel(const Layer
         const long long row = row0 + WAVES * u;
         if (row < end) {
           float y[V];
+          if constexpr (!UPSTREAM) {
 #pragma unroll
-          for (int e = 0; e < V; ++e) { z[u][e] = __builtin_fmaf(p.alpha, z[u][e], bias[e]); }
+            for (int e = 0; e < V; ++e) { z[u][e] = __builtin_fmaf(p.alpha, z[u][e], bias[e]); }
+          }
           LayerValues<FAST>(p, z[u], old[u], y);
 #pragma unroll
           for (int e = 0; e < V; ++e) { sums[e] += y[e]; }
           if (p.c != nullptr) { LayerPiece<T, V>::Store(static_cast<T*>(p.c) + row * p.c_ld + col, inside, y); }
-          if (p.pre != nullptr && !p.gradient) { LayerPiece<T, V>::Store(static_cast<T*>(p.pre) + row * p.pre_ld + col, inside, z[u]); }
+          if (!UPSTREAM && p.pre != nullptr && !p.gradient) { LayerPiece<T, V>::Store(static_cast<T*>(p.pre) + row * p.pre_ld + col, inside, z[u]); }
         }
       }
     }
@@ -132,6 +121,43 @@ __global__ __launch_bounds__(kLayerRowsThreads) void LayerRowsKernel(const Layer
         p.bias_partials[static_cast<long long>(sums_row) * p.m + feature] = sum;
       }
     }
+  }
+}
+
+// One operand to copy: `matrices` matrices of `lines` lines of `length` elements, ld and stride apart, to lines of new_ld
+// elements, one matrix behind the other. lane_shift: a line takes 2^lane_shift lanes, a piece of 16 bytes each and in turn.
+struct LayerAlignOperand {
+  const void* from;
+  void* to;
+  long long ld, stride, new_ld;
+  int length, lines, matrices, lane_shift;
+};
+struct LayerAlignArgs {
+  LayerAlignOperand operand[2];
+  int blocks_of_first;  // the work-groups from this one on copy the second operand
+};
+template <typename T>
+__global__ __launch_bounds__(kLayerRowsThreads) void LayerAlignKernel(const LayerAlignArgs q) {
+  constexpr int V = 16 / sizeof(T);
+  typedef T Loose __attribute__((ext_vector_type(V), aligned(sizeof(T))));
+  typedef T Tight __attribute__((ext_vector_type(V)));
+  const bool second = static_cast<int>(blockIdx.x) >= q.blocks_of_first;
+  const LayerAlignOperand& o = q.operand[second ? 1 : 0];
+  const long long block = second ? blockIdx.x - q.blocks_of_first : blockIdx.x;
+  const long long line = ((block * kLayerRowsThreads + threadIdx.x) >> o.lane_shift);
+  if (line >= static_cast<long long>(o.lines) * o.matrices) { return; }
+  const int matrix = static_cast<int>(line / o.lines), in_matrix = static_cast<int>(line - static_cast<long long>(matrix) * o.lines);
+  const T* from = static_cast<const T*>(o.from) + matrix * o.stride + in_matrix * o.ld;
+  T* to = static_cast<T*>(o.to) + line * o.new_ld;
+  const int lanes = 1 << o.lane_shift;
+  for (int at = (threadIdx.x & (lanes - 1)) * V; at < o.length; at += lanes * V) {
+    Tight piece;
+    if (at + V <= o.length) { piece = __builtin_bit_cast(Tight, *reinterpret_cast<const Loose*>(from + at)); }
+    else {
+#pragma unroll
+      for (int e = 0; e < V; ++e) { piece[e] = (at + e < o.length) ? from[at + e] : T(0.0f); }
+    }
+    *reinterpret_cast<Tight*>(to + at) = piece;
   }
 }
 

@@ -261,30 +261,6 @@ void Xlayer<T>::DoGemmGroupedGradient(const size_t m, const size_t n, const size
 
 template <typename T>
 void Xlayer<T>::Launch(clbh_layer_desc& desc) {
-  // 16-bit operands are fetched in dwords, four bytes at a time: one that starts at an odd element or has an odd leading
-  // dimension (every row, or every group's matrix, then starts at another parity) is copied into an aligned temporary
-  // first, one pass over it. A leading dimension of more than the kernels' offsets hold is handled the same way.
-  std::unique_ptr<StreamScratch> aligned_a, aligned_b;
-  if (desc.upstream == nullptr) {
-    auto copy = 0;
-    if (clbh_layer_operands_fit(&desc, &copy) == 0) {
-      const auto align = [&](const void*& pointer, long long& ld, long long* stride, const bool kcontig, const int extent,
-                             const int matrices, std::unique_ptr<StreamScratch>& place) {
-        const auto one = kcontig ? desc.k : extent, two = kcontig ? extent : desc.k;
-        const auto new_ld = (static_cast<long long>(one) + 7) / 8 * 8, new_stride = new_ld * two;
-        place.reset(new StreamScratch(static_cast<size_t>(new_stride) * matrices * sizeof(T), stream(), "aligned copy of an operand"));
-        CheckDevice(clbh_copy_matrix_batched(static_cast<int>(8 * sizeof(T)), one, two, matrices, pointer, 0, ld,
-                                             (stride != nullptr) ? *stride : 0, nullptr, place->get(), new_ld, new_stride, stream()),
-                    "clbh_copy_matrix_batched");
-        pointer = place->get();
-        ld = new_ld;
-        if (stride != nullptr) { *stride = new_stride; }
-      };
-      const bool by_rows = desc.grouping == CLBH_GROUPS_BY_ROWS;
-      if (copy & 1) { align(desc.a, desc.a_ld, by_rows ? &desc.a_stride : nullptr, desc.a_kcontig != 0, desc.m, by_rows ? desc.groups : 1, aligned_a); }
-      if (copy & 2) { align(desc.b, desc.b_ld, nullptr, desc.b_kcontig != 0, desc.n, 1, aligned_b); }
-    }
-  }
   ApplyLayerOverrides(sizeof(T) == 4 ? Precision::kSingle : Precision::kHalf, desc.tile_variant, desc.split_k);
   std::unique_ptr<StreamScratch> scratch;
   desc.workspace_bytes = clbh_layer_workspace_bytes(&desc);

@@ -309,9 +309,8 @@ typedef struct clbh_layer_desc_ {
   void* workspace;   // clbh_layer_workspace_bytes(desc) bytes, 256-byte aligned
   size_t workspace_bytes;
 } clbh_layer_desc;
-// 16-bit operands are fetched in dwords: 1 when a and b can be (dword-aligned, even leading dimensions and strides, leading
-// dimensions below CLBH_LAYER_MAX_LD), 0 when the caller has to copy the operand that cannot (bit 0: a, bit 1: b of *copy).
-CLBH_API int clbh_layer_operands_fit(const clbh_layer_desc* desc, int* copy);
+// Scratch of one call: sums of K ranges, sums for the bias gradient, aligned copies of operands - 16-bit operands are fetched
+// in dwords, one whose lines start at odd elements (or whose leading dimension is CLBH_LAYER_MAX_LD or more) is copied first.
 CLBH_API size_t clbh_layer_workspace_bytes(const clbh_layer_desc* desc);
 // Enqueues the kernels of one call. Returns 0 or the HIP error code.
 CLBH_API int clbh_layer_launch(const clbh_layer_desc* desc, hipStream_t stream);
