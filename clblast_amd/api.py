@@ -410,29 +410,35 @@ def _layer_function(routine, dtype):
 
 
 def _layer(routine, queue, tensors, group_offsets, arguments):
-    import torch
     first = tensors[0]
-    dtype, device = first.dtype, first.device
+    dtype, device = first.dtype, first.get_device()  # (-1 on the host)
     for t in tensors:
         if t is not None:
             if t.dtype is not dtype:
                 raise ValueError("PyCLBlast: All arrays have to be of the same data-type, got: %s and %s" % (dtype, t.dtype))
-            if t.device != device:
+            if t.get_device() != device:
                 raise ValueError("PyCLBlast: operands must live on one GPU")
-    if not first.is_cuda:
+    if device < 0:
         raise ValueError("PyCLBlast: operands must live on the GPU")
+    torch = _torch()
     if group_offsets is not None:
         if group_offsets.dtype is not torch.int64 or not group_offsets.is_contiguous():
             raise ValueError("PyCLBlast: group_offsets must be contiguous 64-bit integers")
-        if group_offsets.device != device:
+        if group_offsets.get_device() != device:
             raise ValueError("PyCLBlast: operands must live on one GPU")
     stream = torch.cuda.current_stream() if queue is None else queue
-    if stream.device != device or device.index != torch.cuda.current_device():  # (the device of a launch is the current one)
+    # (a launch needs its stream's device to be the current one; the current stream's is)
+    if stream.device_index != device or (queue is not None and torch.cuda.current_device() != device):
         raise ValueError("PyCLBlast: the operands' GPU must be the queue's and the current one")
     function = _layer_functions.get((routine, dtype)) or _layer_function(routine, dtype)
-    status = function(*arguments, _stream_ref(stream.cuda_stream), None)
+    status = function(*arguments, ctypes.byref(ctypes.c_void_p(stream.cuda_stream)), None)
     if status != 0:
         raise CLBlastError("CLBlast%s%s" % (_LAYER_PREFIX[str(dtype)], routine), status)
+
+
+def _torch():
+    import torch
+    return torch
 
 
 def _activation(name):

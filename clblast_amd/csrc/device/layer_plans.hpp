@@ -14,12 +14,19 @@
 
 namespace clbh {
 
-// Tiles (features x rows): number, extents, work-groups that share a compute unit
+// Tiles (features x rows), and what a work-group of one costs: ns per unit of k while it has a compute unit to itself
+// (`alone`), its share when the compute unit is full of them (`full`), and the us that its start and epilogue keep
+// the compute unit from other work (`fixed`). Fitted on an MI355X to forced tiles at 256 .. 8192 x 4096 x 4096 and 8192^2 x 1024; a
+// tile that is alone on half of the compute units runs faster than one on all of them (the 16-bit products run against the
+// power limit), which the smallest tiles' k-walk, bound by latency, does not show.
 struct LayerTile {
   int variant, tile_m, tile_n, per_cu;
+  double alone_16, full_16, fixed_16, alone_32, full_32, fixed_32;
 };
 constexpr LayerTile kLayerTiles[] = {
-    {0, 128, 128, 2}, {1, 256, 256, 1}, {2, 256, 128, 2}, {3, 64, 64, 4}, {4, 128, 32, 4},
+    {0, 128, 128, 2, 9.7, 9.2, 1.5, 61.6, 58.0, 2.0}, {1, 256, 256, 1, 17.0, 24.8, 11.0, 0.0, 0.0, 0.0},
+    {2, 256, 128, 2, 15.0, 14.9, 5.0, 118.0, 112.0, 5.0}, {3, 64, 64, 4, 7.3, 3.95, 0.2, 18.5, 15.1, 0.3},
+    {4, 128, 32, 4, 7.3, 4.5, 0.2, 18.5, 16.0, 0.3},
 };
 constexpr int kLayerTileCount = sizeof(kLayerTiles) / sizeof(kLayerTiles[0]);
 
@@ -61,6 +68,47 @@ inline int LayerRowsChunk(const long long rows, const long long column_blocks) {
 
 inline int LayerVector(const int type) { return type == CLBH_TYPE_FP32 ? 4 : 8; }
 
+// Estimated time in us of `groups` work-groups of a tile that each walk k: rounds of as many as stay resident, the last one with
+// what is left. (256 x 4096 x 4096 in bf16 on 64 x 64 tiles: 35 estimated, 32 measured; 8192 x 8192 x 1024 on 256 x 256: 146 and
+// 137; 1024 x 1024 x 8192 in four ranges on 128 x 128: 37 and 39.)
+inline double LayerCost(const LayerTile& t, const bool wide, const double work_groups, const double k, const int units) {
+  const double alone = (wide ? t.alone_32 : t.alone_16) * k * 1e-3, full = (wide ? t.full_32 : t.full_16) * k * 1e-3;
+  const double fixed = wide ? t.fixed_32 : t.fixed_16;
+  const double slots = static_cast<double>(units) * t.per_cu;
+  const double rounds = static_cast<double>(static_cast<long long>(work_groups / slots));
+  double cost = 5.0 + rounds * t.per_cu * (full + fixed);
+  const double left = (work_groups - rounds * slots) / units;  // work-groups per compute unit in the last round
+  if (left > 0.0) {
+    const double together = static_cast<double>(static_cast<long long>(left + 0.999));
+    cost += std::max(alone, (t.per_cu == 1 ? left : together) * full) + together * fixed;
+  }
+  return cost;
+}
+
+// Tile and K ranges by that estimate; ranges pay for the sums' way through memory and the second kernel. Measured with two
+// kernels against one: 64 x 1024 x 1024 10.9 / 13.2 us, 64 x 4096 x 4096 33 / 17, 1 x 8192 x 4096 33 / 15.4.
+inline void ChooseLayerTile(const clbh_layer_desc& d, const int units, int& variant, int& ranges) {
+  const bool wide = d.type == CLBH_TYPE_FP32;
+  const bool by_rows = d.grouping == CLBH_GROUPS_BY_ROWS, by_depth = d.grouping == CLBH_GROUPS_BY_DEPTH;
+  double best = 0.0;
+  for (const auto& t : kLayerTiles) {
+    if (!LayerTileExists(d.type, t)) { continue; }
+    const double along_m = static_cast<double>((d.m + t.tile_m - 1) / t.tile_m);
+    // (of groups the host knows the number alone: even ones are assumed)
+    const double rows = by_rows ? static_cast<double>((d.n + d.groups - 1) / d.groups) : static_cast<double>(d.n);
+    const double along_n = static_cast<double>(static_cast<long long>((rows + t.tile_n - 1) / t.tile_n)) * (by_rows ? std::min(d.groups, d.n) : 1);
+    const double groups = along_m * along_n * (by_depth ? d.groups : 1);
+    const double k = by_depth ? std::max(1.0, static_cast<double>(d.k) / d.groups) : static_cast<double>(d.k);
+    for (int s = 1; s <= 32; s = (s < 4) ? s + 1 : s + s / 2) {
+      if (s > 1 && (d.grouping != CLBH_GROUPS_NONE || d.k < 256 * s)) { break; }
+      const double sums = static_cast<double>(s) * d.m * d.n;
+      if (s > 1 && sums * 4.0 > 64e6) { break; }
+      const double cost = LayerCost(t, wide, groups * s, k / s, units) + ((s > 1) ? 5.0 + sums * 8.0 / 4e6 : 0.0);
+      if (best == 0.0 || cost < best) { best = cost; variant = t.variant; ranges = s; }
+    }
+  }
+}
+
 inline LayerPlan PlanLayer(const clbh_layer_desc& d, const int units) {
   auto plan = LayerPlan{};
   plan.splits = 1;
@@ -70,23 +118,13 @@ inline LayerPlan PlanLayer(const clbh_layer_desc& d, const int units) {
     return offset;
   };
   if (d.upstream == nullptr) {
-    const auto count = [&](const LayerTile& t) {
-      const long long along_m = (d.m + t.tile_m - 1) / t.tile_m;
-      const long long along_n = (d.grouping == CLBH_GROUPS_BY_ROWS) ? MostGroupTiles(d.n, d.groups, t.tile_n) : (d.n + t.tile_n - 1) / t.tile_n;
-      return along_m * along_n * ((d.grouping == CLBH_GROUPS_BY_DEPTH) ? d.groups : 1);
-    };
-    int variant = 0;
-    const long long rows_per_group = (d.grouping == CLBH_GROUPS_BY_ROWS) ? (d.n + d.groups - 1) / d.groups : d.n;
-    if (rows_per_group <= 32) { variant = 4; }
-    else if (count(kLayerTiles[0]) < 2ll * units) { variant = 3; }
-    else { variant = (count(kLayerTiles[2]) >= 2ll * units) ? 2 : 0; }
+    int variant = 0, wanted = 1;
+    ChooseLayerTile(d, units, variant, wanted);
     if (d.tile_variant >= 0 && d.tile_variant < kLayerTileCount && LayerTileExists(d.type, kLayerTiles[d.tile_variant])) { variant = d.tile_variant; }
     plan.tile = kLayerTiles[variant];
     plan.tiles_m = (d.m + plan.tile.tile_m - 1) / plan.tile.tile_m;
     plan.tiles_n = (d.grouping == CLBH_GROUPS_BY_ROWS) ? MostGroupTiles(d.n, d.groups, plan.tile.tile_n) : (d.n + plan.tile.tile_n - 1) / plan.tile.tile_n;
-    int wanted = 1;
-    const long long tiles = plan.tiles_m * plan.tiles_n, slots = static_cast<long long>(units) * plan.tile.per_cu;
-    if (2 * tiles <= slots && d.k >= 512) { wanted = static_cast<int>(std::min<long long>({slots / tiles, d.k / 256, 16})); }
+    if (variant == d.tile_variant && d.split_k == 0) { wanted = 1; }  // a tile that is forced alone
     if (d.split_k > 0) { wanted = d.split_k; }
     if (d.grouping == CLBH_GROUPS_NONE && wanted > 1) {
       const int chunk = static_cast<int>(((static_cast<long long>(d.k) + wanted - 1) / wanted + 63) / 64 * 64);

@@ -127,15 +127,21 @@ __device__ __forceinline__ bool FindGroupTile(const long long* __restrict__ offs
   return false;
 }
 
-// The group with the rank-th largest range, for up to 64 groups (one per lane; of equal ones the first comes first); rank itself
-// beyond
-__device__ __forceinline__ int GroupOfRank(const long long* __restrict__ offsets, const int groups, const int rows, const int rank,
-                                           const int lane) {
-  if (groups > 64) { return rank; }
-  int count = -1;
+// The group with the rank-th largest range (of equal ones the first comes first), where it begins and how long it is; for up to
+// 64 groups, one per lane. Group number `rank` beyond.
+__device__ __forceinline__ void GroupOfRank(const long long* __restrict__ offsets, const int groups, const int rows, const int rank,
+                                            const int lane, int& group, int& begin, int& length) {
+  if (groups > 64) {
+    group = rank;
+    int end;
+    GroupRange(offsets, group, rows, begin, end);
+    length = end - begin;
+    return;
+  }
+  int first = 0, count = -1;
   if (lane < groups) {
     const long long from = offsets[lane], to = offsets[lane + 1];
-    const int first = static_cast<int>(from < 0 ? 0 : (from > rows ? rows : from));
+    first = static_cast<int>(from < 0 ? 0 : (from > rows ? rows : from));
     count = static_cast<int>(to < first ? 0 : (to > rows ? rows : to) - first);
   }
   int above = 0;
@@ -143,7 +149,9 @@ __device__ __forceinline__ int GroupOfRank(const long long* __restrict__ offsets
     const int other = __builtin_amdgcn_readlane(count, g);
     above += (other > count || (other == count && g < lane)) ? 1 : 0;
   }
-  return __builtin_ctzll(__ballot(lane < groups && above == rank));
+  group = __builtin_ctzll(__ballot(lane < groups && above == rank));
+  begin = __builtin_amdgcn_readlane(first, group);
+  length = __builtin_amdgcn_readlane(count, group);
 }
 
 // ---- types and configurations ------------------------------------------------------------------------------------------
@@ -485,10 +493,7 @@ __global__ __launch_bounds__(Config::THREADS, Config::MIN_WAVES) void LayerGemmK
     const int share = (tiles_m * tiles_n + kNumXcd - 1) / kNumXcd;
     const int local = static_cast<int>(blockIdx.x / kNumXcd) % share + static_cast<int>(blockIdx.x % kNumXcd) * share;
     if (local >= tiles_m * tiles_n) { return; }
-    group = GroupOfRank(p.offsets, p.groups, p.k, blockIdx.x / kNumXcd / share, lane);
-    int end;
-    GroupRange(p.offsets, group, p.k, first, end);
-    depth = end - first;
+    GroupOfRank(p.offsets, p.groups, p.k, blockIdx.x / kNumXcd / share, lane, group, first, depth);
     const int walk = local / (8 * tiles_n), height = min(tiles_m - 8 * walk, 8);
     tile_m = 8 * walk + (local - walk * 8 * tiles_n) % height;
     tile_n = (local - walk * 8 * tiles_n) / height;
