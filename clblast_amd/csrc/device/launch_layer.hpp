@@ -83,16 +83,22 @@ int LaunchLayerConfig(const clbh_layer_desc& d, const LayerPlan& plan, const Lay
   }
 }
 
+// Rings of LDS buffers: as deep as the work-groups that share a compute unit leave room for. 16 bits (512 x 4096 x 4096 on 128 x 128,
+// 256 x 4096 x 4096 on 64 x 64, one work-group per compute unit): ring of three 45 and 32 us, four 36 and 23, five 36 and
+// 21, six - one work-group less fits - 45 and 20. The fp32 walk is bound by its products: 254 and 81 us with any of them.
 template <typename T>
 int LaunchLayerProduct(const clbh_layer_desc& d, const LayerPlan& plan, const LayerArgs& args, hipStream_t stream) {
+  constexpr bool HALF = sizeof(T) == 2;
   switch (plan.tile.variant) {
     case 1:
-      if constexpr (sizeof(T) == 2) { return LaunchLayerConfig<LayerConfig<T, 2, 4, 4, 2, 2>>(d, plan, args, stream); }
+      if constexpr (HALF) { return LaunchLayerConfig<LayerConfig<T, 2, 4, 4, 2, 2>>(d, plan, args, stream); }
       else { return hipErrorInvalidValue; }
     case 2: return LaunchLayerConfig<LayerConfig<T, 2, 2, 4, 2, 2>>(d, plan, args, stream);
-    case 3: return LaunchLayerConfig<LayerConfig<T, 2, 2, 1, 1, 4>>(d, plan, args, stream);
-    case 4: return LaunchLayerConfig<LayerConfig<T, 4, 1, 1, 1, 4>>(d, plan, args, stream);
-    default: return LaunchLayerConfig<LayerConfig<T, 2, 2, 2, 2, 2>>(d, plan, args, stream);
+    case 3: return LaunchLayerConfig<LayerConfig<T, 2, 2, 1, 1, 4, HALF ? 5 : 3>>(d, plan, args, stream);
+    case 4:
+      if constexpr (!HALF) { return LaunchLayerConfig<LayerConfig<T, 4, 1, 1, 1, 4>>(d, plan, args, stream); }
+      else { return hipErrorInvalidValue; }
+    default: return LaunchLayerConfig<LayerConfig<T, 2, 2, 2, 2, 2, HALF ? 4 : 3>>(d, plan, args, stream);
   }
 }
 

@@ -24,9 +24,9 @@ struct LayerTile {
   double alone_16, full_16, fixed_16, alone_32, full_32, fixed_32;
 };
 constexpr LayerTile kLayerTiles[] = {
-    {0, 128, 128, 2, 9.7, 9.2, 1.5, 61.6, 58.0, 2.0}, {1, 256, 256, 1, 17.0, 24.8, 11.0, 0.0, 0.0, 0.0},
-    {2, 256, 128, 2, 15.0, 14.9, 5.0, 118.0, 112.0, 5.0}, {3, 64, 64, 4, 7.3, 3.95, 0.2, 18.5, 15.1, 0.3},
-    {4, 128, 32, 4, 7.3, 4.5, 0.2, 18.5, 16.0, 0.3},
+    {0, 128, 128, 2, 7.3, 8.6, 1.5, 61.6, 58.0, 2.0}, {1, 256, 256, 1, 17.0, 24.8, 8.0, 0.0, 0.0, 0.0},
+    {2, 256, 128, 2, 15.0, 14.9, 4.0, 118.0, 112.0, 5.0}, {3, 64, 64, 4, 4.1, 3.7, 0.2, 18.5, 15.1, 0.3},
+    {4, 128, 32, 4, 0.0, 0.0, 0.0, 18.5, 16.0, 0.3},
 };
 constexpr int kLayerTileCount = sizeof(kLayerTiles) / sizeof(kLayerTiles[0]);
 
@@ -55,7 +55,7 @@ inline long long MostGroupTiles(const long long rows, const long long groups, co
 }
 
 inline bool LayerTileExists(const int type, const LayerTile& tile) {
-  return type != CLBH_TYPE_FP32 || tile.variant != 1;
+  return (type == CLBH_TYPE_FP32) ? tile.full_32 > 0.0 : tile.full_16 > 0.0;
 }
 
 // Rows per work-group of the elementwise kernel: as few as give about 2048 work-groups, at least 8 (two per wavefront), at

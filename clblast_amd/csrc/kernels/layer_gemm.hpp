@@ -12,7 +12,7 @@
 // The offsets lie in device memory; they are clamped to the rows that exist, so no offset leads outside a matrix.
 //
 // Structure: a work-group owns a TILE_M x TILE_N tile, K is walked in slabs of 64 bytes per line (32 halfs, 16 floats) in a
-// ring of three LDS buffers. Both types share the byte layout of a slab, the direct global -> LDS requests (16 bytes per lane, range-checked
+// ring of LDS buffers. Both types share the byte layout of a slab, the direct global -> LDS requests (16 bytes per lane, range-checked
 // by the buffer resource), the one barrier per slab and the order of products: the wavefront's blocks form four quadrants
 // whose missing fragments are read under the products of the quadrant before. What differs is the instruction: 16 bits
 // v_mfma_f32_16x16x32_{f16,bf16}, a slab is one instruction deep, and x-contiguous operands are read with the transposing LDS
@@ -162,7 +162,7 @@ typedef float layer_float4_t __attribute__((ext_vector_type(4)));
 typedef float layer_float8_t __attribute__((ext_vector_type(8)));
 
 // WM x WN wavefronts, each owning (32 FM) x (32 FN) of the tile; BLOCK: extent of the matrix instruction's block.
-template <typename T_, int WM_, int WN_, int FM_, int FN_, int MIN_WAVES_>
+template <typename T_, int WM_, int WN_, int FM_, int FN_, int MIN_WAVES_, int STAGES_ = 3>
 struct LayerConfig {
   using T = T_;
   static constexpr int WM = WM_, WN = WN_, FM = FM_, FN = FN_, MIN_WAVES = MIN_WAVES_;
@@ -172,7 +172,7 @@ struct LayerConfig {
   static constexpr int VEC = 16 / sizeof(T);
   static constexpr int BLOCK = (sizeof(T) == 4 && FM % 2 == 0 && FN % 2 == 0) ? 32 : 16;
   static constexpr int BM = 32 * FM / BLOCK, BN = 32 * FN / BLOCK;  // the wavefront's blocks
-  static constexpr int STAGES = 3;
+  static constexpr int STAGES = STAGES_;  // LDS slab buffers: slab + STAGES - 1 is requested under the products of a slab
   static constexpr int PIECES_A = TILE_M / 16, PIECES_B = TILE_N / 16;  // 1 KiB pieces of a slab
   static constexpr int ROUNDS = (PIECES_A + PIECES_B + WAVES - 1) / WAVES;
   static constexpr bool DUMMY = (PIECES_A + PIECES_B) % WAVES != 0;
@@ -310,29 +310,39 @@ __device__ __forceinline__ void LayerZeroTail(char* stage, const int piece, cons
 
 // V values through the layer's elementwise work: z is alpha times the sum (+ bias), `other` the residual (forward) or Z
 // (gradient). The choices are the launch's; they stand outside the loops over the values.
-template <bool FAST, int ACTIVATION, int V>
+// OTHER: there is such a value (without one a gradient has no activation to go through)
+template <bool FAST, int ACTIVATION, bool OTHER, int V>
 __device__ __forceinline__ void LayerValuesOf(const LayerArgs& p, const float (&z)[V], const float (&other)[V], float (&y)[V]) {
-  if (p.gradient) {
+  if (OTHER && p.gradient) {
 #pragma unroll
     for (int e = 0; e < V; ++e) { y[e] = z[e] * ActivationSlope<FAST>(ACTIVATION, other[e]); }
   } else {
 #pragma unroll
     for (int e = 0; e < V; ++e) { y[e] = Activate<FAST>(ACTIVATION, z[e]); }
-    if (p.beta != 0.0f) {
+    if (OTHER && p.beta != 0.0f) {
 #pragma unroll
       for (int e = 0; e < V; ++e) { y[e] = __builtin_fmaf(p.beta, other[e], y[e]); }
     }
   }
 }
-template <bool FAST, int V>
+template <bool FAST, bool OTHER, int V>
 __device__ __forceinline__ void LayerValues(const LayerArgs& p, const float (&z)[V], const float (&other)[V], float (&y)[V]) {
   switch (p.activation) {
-    case kActivationRelu: LayerValuesOf<FAST, kActivationRelu>(p, z, other, y); break;
-    case kActivationGelu: LayerValuesOf<FAST, kActivationGelu>(p, z, other, y); break;
-    case kActivationGeluTanh: LayerValuesOf<FAST, kActivationGeluTanh>(p, z, other, y); break;
-    case kActivationSilu: LayerValuesOf<FAST, kActivationSilu>(p, z, other, y); break;
-    default: LayerValuesOf<FAST, kActivationNone>(p, z, other, y); break;
+    case kActivationRelu: LayerValuesOf<FAST, kActivationRelu, OTHER>(p, z, other, y); break;
+    case kActivationGelu: LayerValuesOf<FAST, kActivationGelu, OTHER>(p, z, other, y); break;
+    case kActivationGeluTanh: LayerValuesOf<FAST, kActivationGeluTanh, OTHER>(p, z, other, y); break;
+    case kActivationSilu: LayerValuesOf<FAST, kActivationSilu, OTHER>(p, z, other, y); break;
+    default: LayerValuesOf<FAST, kActivationNone, OTHER>(p, z, other, y); break;
   }
+}
+
+// A global address that is the same in all lanes, in scalar registers whatever the compiler thinks of how it came about
+typedef __attribute__((address_space(1))) char* GlobalBytes;
+__device__ __forceinline__ GlobalBytes UniformAddress(const void* pointer) {
+  const unsigned long long address = reinterpret_cast<unsigned long long>(pointer);
+  const unsigned long long low = static_cast<unsigned>(__builtin_amdgcn_readfirstlane(static_cast<int>(address)));
+  const unsigned long long high = static_cast<unsigned>(__builtin_amdgcn_readfirstlane(static_cast<int>(address >> 32)));
+  return (GlobalBytes)((high << 32) | low);
 }
 
 // V consecutive values of a row, of which the first `inside` exist, as one access at whatever address the row starts (the
@@ -340,6 +350,20 @@ __device__ __forceinline__ void LayerValues(const LayerArgs& p, const float (&z)
 template <typename T, int V>
 struct LayerPiece {
   typedef T Piece __attribute__((ext_vector_type(V), aligned(sizeof(T))));
+  typedef T Raw __attribute__((ext_vector_type(V)));  // as it is in memory: half the registers of its values for 16 bits
+  static __device__ __forceinline__ void Values(const Raw raw, float (&values)[V]) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) { const T value = raw[e]; values[e] = static_cast<float>(value); }
+  }
+  // at a uniform address and a lane's byte offset from there (the access carries both, no address is computed)
+  typedef __attribute__((address_space(1))) Piece* GlobalPiece;
+  static __device__ __forceinline__ Raw LoadAt(const GlobalBytes base, const unsigned offset) { return *(GlobalPiece)(base + offset); }
+  static __device__ __forceinline__ void StoreAt(const GlobalBytes base, const unsigned offset, const float (&values)[V]) {
+    Piece piece;
+#pragma unroll
+    for (int e = 0; e < V; ++e) { piece[e] = static_cast<T>(values[e]); }
+    *(GlobalPiece)(base + offset) = piece;
+  }
   static __device__ __forceinline__ void Load(const T* from, const int inside, float (&values)[V]) {
     if (inside >= V) {
       const Piece piece = *reinterpret_cast<const Piece*>(from);
@@ -363,8 +387,8 @@ struct LayerPiece {
   }
 };
 
-// Moves staged rows of a wavefront through the epilogue, lanes along the features in pieces of V values. The loop over
-// the rows is not unrolled (its body holds every activation); what it reads from memory is asked for two passes ahead.
+// Moves staged rows of a wavefront through the epilogue, lanes along the features in pieces of V values. The loops over the
+// rows are not unrolled (their bodies hold every activation).
 template <typename Config>
 struct LayerRows {
   using T = typename Config::T;
@@ -391,43 +415,105 @@ struct LayerRows {
   // the first of them
   __device__ __forceinline__ void Run(const LayerArgs& p, const float* stage, T* c, T* pre, const T* other, const long long other_ld,
                                       const int lane, const int rows, const int inside) {
-    constexpr int AHEAD = PASSES < 2 ? PASSES : 2;
-    const int row0 = lane / ROW_LANES, col = V * (lane % ROW_LANES);
-    const auto inside_of = [&](const int row) { return (row < rows) ? inside - col : 0; };
-    float old[AHEAD][V];
-#pragma unroll
-    for (int u = 0; u < AHEAD; ++u) {
-#pragma unroll
-      for (int e = 0; e < V; ++e) { old[u][e] = 0.0f; }
-      const int row = row0 + u * ROWS;
-      if (other != nullptr) { Piece::Load(other + row * other_ld + col, inside_of(row), old[u]); }
+    T* z_out = p.gradient ? nullptr : pre;
+    // (a lane's offset within a pass, up to 16 rows, in 32 bits)
+    const bool small = p.c_ld < (1 << 25) && (z_out == nullptr || p.pre_ld < (1 << 25)) && (other == nullptr || other_ld < (1 << 25));
+    if (rows >= Config::HALF_N && inside >= Config::WAVE_M && small) {
+      if (other != nullptr) { Whole<true>(p, stage, c, z_out, other, other_ld, lane); }
+      else { Whole<false>(p, stage, c, z_out, other, other_ld, lane); }
+    } else {
+      Partial(p, stage, c, z_out, other, other_ld, lane, rows, inside);
     }
-#pragma unroll 1
-    for (int pass = 0; pass < PASSES; pass += AHEAD) {
+  }
+
+  static constexpr int FOURS = V / 4;
+  static __device__ __forceinline__ void Fetch(const float* from, layer_float4_t (&staged)[FOURS]) {
+#pragma unroll
+    for (int q = 0; q < FOURS; ++q) { staged[q] = *reinterpret_cast<const layer_float4_t*>(from + 4 * q); }
+  }
+  __device__ __forceinline__ void Scale(const LayerArgs& p, const layer_float4_t (&staged)[FOURS], float (&z)[V]) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) { z[e] = __builtin_fmaf(p.alpha, staged[e / 4][e % 4], bias[e]); }
+  }
+
+  // All rows and features exist. Nothing but the values is left to the vector unit: addresses advance as scalars. (With them
+  // and the tests for partial pieces in vector registers the pass took 4.6 of a 256 x 256 tile's 12 us.)
+  template <bool OTHER>
+  __device__ __forceinline__ void Whole(const LayerArgs& p, const float* stage, T* c, T* z_out, const T* other, const long long other_ld,
+                                        const int lane) {
+    constexpr int AHEAD = PASSES < 4 ? PASSES : 4;  // passes that `other` is asked for in advance
+    constexpr unsigned SIZE = sizeof(T);
+    const int row0 = lane / ROW_LANES, col = V * (lane % ROW_LANES);
+    const auto offset = [&](const long long ld) { return (static_cast<unsigned>(row0) * static_cast<unsigned>(ld) + col) * SIZE; };
+    GlobalBytes c_base = UniformAddress(c);
+    GlobalBytes z_base = UniformAddress(z_out);
+    GlobalBytes other_base = UniformAddress(other);
+    const unsigned c_offset = offset(p.c_ld), z_offset = offset(p.pre_ld), other_offset = offset(other_ld);
+    const long long c_step = ROWS * p.c_ld * SIZE, z_step = ROWS * p.pre_ld * SIZE, other_step = ROWS * other_ld * SIZE;
+    typename Piece::Raw old[AHEAD];
+    if constexpr (OTHER) {
 #pragma unroll
       for (int u = 0; u < AHEAD; ++u) {
-        const int row = row0 + (pass + u) * ROWS;
-        float now[V], z[V], y[V];
-#pragma unroll
-        for (int e = 0; e < V; ++e) { now[e] = old[u][e]; }
-        const int next = row + AHEAD * ROWS;
-        if (other != nullptr) { Piece::Load(other + next * other_ld + col, pass + u + AHEAD < PASSES ? inside_of(next) : 0, old[u]); }
-        const float* from = stage + row * Config::PITCH + col;
-#pragma unroll
-        for (int q = 0; q < V; q += 4) {
-          const layer_float4_t four = *reinterpret_cast<const layer_float4_t*>(from + q);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) { z[q + e] = __builtin_fmaf(p.alpha, four[e], bias[q + e]); }
-        }
-        LayerValues<FAST>(p, z, now, y);
-        const int here = inside_of(row);
-        if (here > 0) {
-#pragma unroll
-          for (int e = 0; e < V; ++e) { sums[e] += y[e]; }
-        }
-        Piece::Store(c + row * p.c_ld + col, here, y);
-        if (pre != nullptr && !p.gradient) { Piece::Store(pre + row * p.pre_ld + col, here, z); }
+        old[u] = Piece::LoadAt(other_base, other_offset);
+        other_base += other_step;
       }
+    }
+    const float* from = stage + row0 * Config::PITCH + col;
+    layer_float4_t staged[FOURS];
+    Fetch(from, staged);
+#pragma unroll 1
+    for (int pass = 0; pass < PASSES; ++pass) {
+      float now[V], z[V], y[V];
+      Scale(p, staged, z);
+      if (pass + 1 < PASSES) { from += ROWS * Config::PITCH; }
+      Fetch(from, staged);  // (of the next pass: its latency under this one's arithmetic)
+      if constexpr (OTHER) {
+        Piece::Values(old[0], now);
+#pragma unroll
+        for (int u = 0; u + 1 < AHEAD; ++u) { old[u] = old[u + 1]; }
+        if (pass + AHEAD < PASSES) { old[AHEAD - 1] = Piece::LoadAt(other_base, other_offset); }
+        other_base += other_step;
+      }
+      LayerValues<FAST, OTHER>(p, z, now, y);
+      if (p.bias_partials != nullptr) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) { sums[e] += y[e]; }
+      }
+      Piece::StoreAt(c_base, c_offset, y);
+      c_base += c_step;
+      if (z_out != nullptr) {
+        Piece::StoreAt(z_base, z_offset, z);
+        z_base += z_step;
+      }
+    }
+  }
+
+  // A tile at the edge of the matrix or of a group
+  __device__ __forceinline__ void Partial(const LayerArgs& p, const float* stage, T* c, T* z_out, const T* other, const long long other_ld,
+                                          const int lane, const int rows, const int inside) {
+    const int row0 = lane / ROW_LANES, col = V * (lane % ROW_LANES);
+    const auto inside_of = [&](const int row) { return (row < rows) ? inside - col : 0; };
+    float next[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) { next[e] = 0.0f; }
+    if (other != nullptr) { Piece::Load(other + row0 * other_ld + col, inside_of(row0), next); }
+#pragma unroll 1
+    for (int pass = 0; pass < PASSES; ++pass) {
+      const int row = row0 + pass * ROWS, here = inside_of(row);
+      float now[V], z[V], y[V];
+#pragma unroll
+      for (int e = 0; e < V; ++e) { now[e] = next[e]; }
+      if (other != nullptr && pass + 1 < PASSES) { Piece::Load(other + (row + ROWS) * other_ld + col, inside_of(row + ROWS), next); }
+      layer_float4_t staged[FOURS];
+      Fetch(stage + row * Config::PITCH + col, staged);
+      Scale(p, staged, z);
+      LayerValues<FAST, true>(p, z, now, y);
+      if (here > 0) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) { sums[e] += y[e]; }
+      }
+      Piece::Store(c + row * p.c_ld + col, here, y);
+      if (z_out != nullptr) { Piece::Store(z_out + row * p.pre_ld + col, here, z); }
     }
   }
 
@@ -455,6 +541,7 @@ __global__ __launch_bounds__(Config::THREADS, Config::MIN_WAVES) void LayerGemmK
   constexpr int TILE_M = Config::TILE_M, TILE_N = Config::TILE_N, TILE_K = Config::TILE_K, BLOCK = Config::BLOCK;
   constexpr int BM = Config::BM, BN = Config::BN, HM = BM / 2, HN = BN / 2;
   constexpr int WAVES = Config::WAVES, ROUNDS = Config::ROUNDS, STAGES = Config::STAGES, AHEAD = STAGES - 1;
+  static_assert(AHEAD >= 2 && AHEAD <= 5 && AHEAD * ROUNDS < 64, "the waits below");
   using KernelTag = std::tuple<Config, std::integral_constant<int, (A_KC ? 2 : 0) | (B_KC ? 1 : 0)>>;
 
   extern __shared__ __align__(16) unsigned char lds_raw[];
@@ -612,7 +699,10 @@ __global__ __launch_bounds__(Config::THREADS, Config::MIN_WAVES) void LayerGemmK
         }
       }
       if (first_slabs == 1) { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
-      else { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(ROUNDS) : "memory"); }
+      else if (first_slabs == 2) { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(ROUNDS) : "memory"); }
+      else if (first_slabs == 3) { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * ROUNDS) : "memory"); }
+      else if (first_slabs == 4) { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(3 * ROUNDS) : "memory"); }
+      else { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(4 * ROUNDS) : "memory"); }
       if (slabs == 1) { zero_tail(0); }
       __syncthreads();
       Frag a_frag[2][HM], b_frag[2][HN];
@@ -621,7 +711,7 @@ __global__ __launch_bounds__(Config::THREADS, Config::MIN_WAVES) void LayerGemmK
 #pragma unroll
       for (int q = 0; q < HN; ++q) { b_frag[0][q] = read_b(b_ring, q); }
       int cur = 0;
-      // One slab; LATER: how many follow it, capped at AHEAD. Slab + 2 is requested under the first two quadrants, into the
+      // One slab; LATER: how many follow it, capped at AHEAD. Slab + AHEAD is requested under the first two quadrants, into the
       // buffer whose reads everybody had waited for at the previous barrier.
       constexpr int PER_SLOT = (ROUNDS + 2 * HM - 1) / (2 * HM);
       const auto slab_body = [&](auto later_tag) {
@@ -662,8 +752,8 @@ __global__ __launch_bounds__(Config::THREADS, Config::MIN_WAVES) void LayerGemmK
             __builtin_amdgcn_sched_barrier(0);
           }
           if (quadrant == 1) {
-            // slab + 1 must have landed for everybody; the requests for the slab behind it may stay in flight
-            constexpr int IN_FLIGHT = (LATER >= 2) ? ROUNDS : 0;
+            // slab + 1 must have landed for everybody; the requests for the slabs behind it may stay in flight
+            constexpr int IN_FLIGHT = (LATER >= 2) ? (LATER - 1) * ROUNDS : 0;
             asm volatile("s_waitcnt vmcnt(%0)" ::"n"(IN_FLIGHT) : "memory");
             if (LATER == 1) { zero_tail(nxt); }  // slab + 1 is the last one
             asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
@@ -677,8 +767,15 @@ __global__ __launch_bounds__(Config::THREADS, Config::MIN_WAVES) void LayerGemmK
       };
       int slab = 0;
       for (; slab + AHEAD < slabs; ++slab) { slab_body(std::integral_constant<int, AHEAD>{}); }
-      if (slab + 1 < slabs) { slab_body(std::integral_constant<int, 1>{}); ++slab; }
-      slab_body(std::integral_constant<int, 0>{});
+      const auto last_slabs = [&](auto self, auto later_tag) {
+        constexpr int LATER = decltype(later_tag)::value;
+        if (slab + LATER < slabs) {
+          slab_body(later_tag);
+          ++slab;
+        }
+        if constexpr (LATER > 0) { self(self, std::integral_constant<int, LATER - 1>{}); }
+      };
+      last_slabs(last_slabs, std::integral_constant<int, AHEAD - 1>{});
     };
     if (m0 + TILE_M <= p.m && n0 + TILE_N <= rows && k_tail == 0) { walk(std::false_type{}); }
     else { walk(std::true_type{}); }

@@ -99,7 +99,7 @@ __global__ __launch_bounds__(kLayerRowsThreads, UPSTREAM ? 5 : 4) void LayerRows
 #pragma unroll
             for (int e = 0; e < V; ++e) { z[u][e] = __builtin_fmaf(p.alpha, z[u][e], bias[e]); }
           }
-          LayerValues<FAST>(p, z[u], old[u], y);
+          LayerValues<FAST, true>(p, z[u], old[u], y);
 #pragma unroll
           for (int e = 0; e < V; ++e) { sums[e] += y[e]; }
           if (p.c != nullptr) { LayerPiece<T, V>::Store(static_cast<T*>(p.c) + row * p.c_ld + col, inside, y); }
