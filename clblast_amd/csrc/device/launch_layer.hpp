@@ -93,7 +93,9 @@ int LaunchLayerProduct(const clbh_layer_desc& d, const LayerPlan& plan, const La
     case 1:
       if constexpr (HALF) { return LaunchLayerConfig<LayerConfig<T, 2, 4, 4, 2, 2>>(d, plan, args, stream); }
       else { return hipErrorInvalidValue; }
-    case 2: return LaunchLayerConfig<LayerConfig<T, 2, 2, 4, 2, 2>>(d, plan, args, stream);
+    case 2:
+      if constexpr (HALF) { return LaunchLayerConfig<LayerConfig<T, 2, 2, 4, 2, 2>>(d, plan, args, stream); }
+      else { return hipErrorInvalidValue; }
     case 3: return LaunchLayerConfig<LayerConfig<T, 2, 2, 1, 1, 4, HALF ? 5 : 3>>(d, plan, args, stream);
     case 4:
       if constexpr (!HALF) { return LaunchLayerConfig<LayerConfig<T, 4, 1, 1, 1, 4>>(d, plan, args, stream); }

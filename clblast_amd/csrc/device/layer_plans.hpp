@@ -25,7 +25,7 @@ struct LayerTile {
 };
 constexpr LayerTile kLayerTiles[] = {
     {0, 128, 128, 2, 7.3, 8.6, 1.5, 61.6, 58.0, 2.0}, {1, 256, 256, 1, 17.0, 24.8, 8.0, 0.0, 0.0, 0.0},
-    {2, 256, 128, 2, 15.0, 14.9, 4.0, 118.0, 112.0, 5.0}, {3, 64, 64, 4, 4.1, 3.7, 0.2, 18.5, 15.1, 0.3},
+    {2, 256, 128, 2, 15.0, 14.9, 4.0, 0.0, 0.0, 0.0}, {3, 64, 64, 4, 4.1, 3.7, 0.2, 16.8, 14.6, 0.3},
     {4, 128, 32, 4, 0.0, 0.0, 0.0, 18.5, 16.0, 0.3},
 };
 constexpr int kLayerTileCount = sizeof(kLayerTiles) / sizeof(kLayerTiles[0]);

@@ -33,21 +33,21 @@ __device__ __forceinline__ float Reciprocal(const float x) {
   return FAST ? __builtin_amdgcn_rcpf(x) : 1.0f / x;
 }
 
-// Phi(z); `bell` receives exp(-z^2 / 2)
+// Phi(-|z|); `bell` receives exp(-z^2 / 2)
 template <bool FAST>
-__device__ __forceinline__ float NormalDistribution(const float z, float& bell) {
-  bell = Exponential<FAST>(-0.5f * z * z);
+__device__ __forceinline__ float NormalTail(const float z, float& bell) {
   if constexpr (FAST) {
+    bell = __builtin_amdgcn_exp2f(-0.72134752f * z * z);  // -log2(e) / 2
     const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.43f * 0.70710678f, __builtin_fabsf(z), 1.0f));
-    float q = __builtin_fmaf(-0.15338767f, t, 0.40704837f);
-    q = __builtin_fmaf(q, t, -0.01078906f);
-    q = __builtin_fmaf(q, t, 0.28136584f);
-    q = __builtin_fmaf(q, t, 0.23251006f);
-    q = __builtin_fmaf(q, t, 0.24325760f);
-    const float tail = 0.5f * (q * t) * bell;
-    return (z > 0.0f) ? 1.0f - tail : tail;
+    float q = __builtin_fmaf(0.5f * -0.15338767f, t, 0.5f * 0.40704837f);
+    q = __builtin_fmaf(q, t, 0.5f * -0.01078906f);
+    q = __builtin_fmaf(q, t, 0.5f * 0.28136584f);
+    q = __builtin_fmaf(q, t, 0.5f * 0.23251006f);
+    q = __builtin_fmaf(q, t, 0.5f * 0.24325760f);
+    return q * t * bell;
   } else {
-    return 0.5f * erfcf(-0.70710678f * z);
+    bell = expf(-0.5f * z * z);
+    return 0.5f * erfcf(0.70710678f * __builtin_fabsf(z));
   }
 }
 
@@ -58,7 +58,11 @@ template <bool FAST>
 __device__ __forceinline__ float Activate(const int activation, const float z) {
   switch (activation) {
     case kActivationRelu: return (z < 0.0f) ? 0.0f : z;  // (a NaN stays one)
-    case kActivationGelu: { float bell; return z * NormalDistribution<FAST>(z, bell); }
+    case kActivationGelu: {  // z Phi(z): z - z Phi(-z) on the positive side, z Phi(-|z|) on the other
+      float bell;
+      const float tail = NormalTail<FAST>(z, bell);
+      return __builtin_fmaf(-__builtin_fabsf(z), tail, (z < 0.0f) ? 0.0f : z);  // (a NaN stays one)
+    }
     case kActivationGeluTanh: {
       const float u = kTanhSlope * z * __builtin_fmaf(0.044715f * z, z, 1.0f);
       return z * Reciprocal<FAST>(1.0f + Exponential<FAST>(-2.0f * u));
@@ -75,8 +79,8 @@ __device__ __forceinline__ float ActivationSlope(const int activation, const flo
     case kActivationRelu: return (z > 0.0f) ? 1.0f : 0.0f;
     case kActivationGelu: {
       float bell;
-      const float phi = NormalDistribution<FAST>(z, bell);
-      return __builtin_fmaf(0.39894228f * z, bell, phi);  // 1 / sqrt(2 pi)
+      const float tail = NormalTail<FAST>(z, bell);
+      return __builtin_fmaf(0.39894228f * z, bell, (z > 0.0f) ? 1.0f - tail : tail);  // 1 / sqrt(2 pi)
     }
     case kActivationGeluTanh: {
       const float u = kTanhSlope * z * __builtin_fmaf(0.044715f * z, z, 1.0f);

@@ -237,10 +237,9 @@ struct LayerMath32<Config, 32> {
     }
     return out;
   }
-  static __device__ __forceinline__ Acc Multiply(const Frag a, const Frag b, Acc acc) {
-#pragma unroll
-    for (int s = 0; s < 8; ++s) { acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a[s], b[s], acc, 0, 0, 0); }
-    return acc;
+  static constexpr int STEPS = 8;  // instructions per block and slab
+  static __device__ __forceinline__ Acc Step(const Frag a, const Frag b, const Acc acc, const int s) {
+    return __builtin_amdgcn_mfma_f32_32x32x2f32(a[s], b[s], acc, 0, 0, 0);
   }
 };
 template <typename Config>
@@ -261,10 +260,9 @@ struct LayerMath32<Config, 16> {
     for (int s = 0; s < 4; ++s) { out[s] = from[s * W]; }
     return out;
   }
-  static __device__ __forceinline__ Acc Multiply(const Frag a, const Frag b, Acc acc) {
-#pragma unroll
-    for (int s = 0; s < 4; ++s) { acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a[s], b[s], acc, 0, 0, 0); }
-    return acc;
+  static constexpr int STEPS = 4;
+  static __device__ __forceinline__ Acc Step(const Frag a, const Frag b, const Acc acc, const int s) {
+    return __builtin_amdgcn_mfma_f32_16x16x4f32(a[s], b[s], acc, 0, 0, 0);
   }
 };
 
@@ -346,7 +344,8 @@ __device__ __forceinline__ GlobalBytes UniformAddress(const void* pointer) {
 }
 
 // V consecutive values of a row, of which the first `inside` exist, as one access at whatever address the row starts (the
-// hardware splits one that is not aligned)
+// hardware splits one that is not aligned). Results are stored past the caches' keeping: they are not read again here and would push
+// out the operands that neighbouring tiles share (8192 x 8192 x 1024 142 -> 121 us, x 4096 with GELU and Z 476 -> 462 us).
 template <typename T, int V>
 struct LayerPiece {
   typedef T Piece __attribute__((ext_vector_type(V), aligned(sizeof(T))));
@@ -362,11 +361,15 @@ struct LayerPiece {
     Piece piece;
 #pragma unroll
     for (int e = 0; e < V; ++e) { piece[e] = static_cast<T>(values[e]); }
-    *(GlobalPiece)(base + offset) = piece;
+    __builtin_nontemporal_store(piece, (GlobalPiece)(base + offset));
   }
+  // STREAM: what nobody reads a second time
+  template <bool STREAM = false>
   static __device__ __forceinline__ void Load(const T* from, const int inside, float (&values)[V]) {
     if (inside >= V) {
-      const Piece piece = *reinterpret_cast<const Piece*>(from);
+      Piece piece;
+      if constexpr (STREAM) { piece = __builtin_nontemporal_load(reinterpret_cast<const Piece*>(from)); }
+      else { piece = *reinterpret_cast<const Piece*>(from); }
 #pragma unroll
       for (int e = 0; e < V; ++e) { const T value = piece[e]; values[e] = static_cast<float>(value); }
     } else {
@@ -379,7 +382,7 @@ struct LayerPiece {
       Piece piece;
 #pragma unroll
       for (int e = 0; e < V; ++e) { piece[e] = static_cast<T>(values[e]); }
-      *reinterpret_cast<Piece*>(to) = piece;
+      __builtin_nontemporal_store(piece, reinterpret_cast<Piece*>(to));
     } else {
 #pragma unroll
       for (int e = 0; e < V; ++e) { if (e < inside) { to[e] = static_cast<T>(values[e]); } }
@@ -705,23 +708,61 @@ __global__ __launch_bounds__(Config::THREADS, Config::MIN_WAVES) void LayerGemmK
       else { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(4 * ROUNDS) : "memory"); }
       if (slabs == 1) { zero_tail(0); }
       __syncthreads();
-      Frag a_frag[2][HM], b_frag[2][HN];
+      // 16 bits: halves of the fragments of one slab; fp32: all fragments of two slabs
+      constexpr bool WIDE = sizeof(T) == 4;
+      Frag a_frag[2][WIDE ? BM : HM], b_frag[2][WIDE ? BN : HN];
 #pragma unroll
-      for (int q = 0; q < HM; ++q) { a_frag[0][q] = read_a(a_ring, q); }
+      for (int q = 0; q < (WIDE ? BM : HM); ++q) { a_frag[0][q] = read_a(a_ring, q); }
 #pragma unroll
-      for (int q = 0; q < HN; ++q) { b_frag[0][q] = read_b(b_ring, q); }
+      for (int q = 0; q < (WIDE ? BN : HN); ++q) { b_frag[0][q] = read_b(b_ring, q); }
       int cur = 0;
       // One slab; LATER: how many follow it, capped at AHEAD. Slab + AHEAD is requested under the first two quadrants, into the
       // buffer whose reads everybody had waited for at the previous barrier.
       constexpr int PER_SLOT = (ROUNDS + 2 * HM - 1) / (2 * HM);
-      const auto slab_body = [&](auto later_tag) {
+      const auto slab_body = [&](auto later_tag, auto parity_tag) {
         constexpr int LATER = decltype(later_tag)::value;
+        constexpr int PARITY = decltype(parity_tag)::value;  // fp32: which set of fragments holds the slab
         constexpr bool LOAD = LATER == AHEAD;
         const int nxt = (cur == STAGES - 1) ? 0 : cur + 1, prv = (cur == 0) ? STAGES - 1 : cur - 1;
         const char* a_cur = a_ring + cur * Config::A_BYTES;
         const char* b_cur = b_ring + cur * Config::B_BYTES;
         const char* a_nxt = a_ring + nxt * Config::A_BYTES;
         const char* b_nxt = b_ring + nxt * Config::B_BYTES;
+        const auto next_slab_in_place = [&]() {
+          // slab + 1 must have landed for everybody; the requests for the slabs behind it may stay in flight
+          constexpr int IN_FLIGHT = (LATER >= 2) ? (LATER - 1) * ROUNDS : 0;
+          asm volatile("s_waitcnt vmcnt(%0)" ::"n"(IN_FLIGHT) : "memory");
+          if (LATER == 1) { zero_tail(nxt); }  // slab + 1 is the last one
+          asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        };
+        if constexpr (WIDE) {
+          // fp32: all blocks between two products into the same registers (block by block the 16x16x4 form of 64 x 64 tiles
+          // loses a tenth); requests under the first half of the slab's steps, the next slab's fragments read under the second
+          constexpr int STEPS = Math::STEPS, PER_STEP = (ROUNDS + STEPS / 2 - 1) / (STEPS / 2);
+#pragma unroll
+          for (int step = 0; step < STEPS; ++step) {
+            if (step == STEPS / 2) {
+              next_slab_in_place();
+#pragma unroll
+              for (int q = 0; q < BM; ++q) { a_frag[1 - PARITY][q] = read_a(a_nxt, q); }
+#pragma unroll
+              for (int q = 0; q < BN; ++q) { b_frag[1 - PARITY][q] = read_b(b_nxt, q); }
+            }
+#pragma unroll
+            for (int i = 0; i < BM; ++i) {
+#pragma unroll
+              for (int j = 0; j < BN; ++j) { acc[i][j] = Math::Step(a_frag[PARITY][i], b_frag[PARITY][j], acc[i][j], step); }
+            }
+            if (LOAD && step < STEPS / 2) {
+#pragma unroll
+              for (int u = 0; u < PER_STEP; ++u) {
+                const int round = step * PER_STEP + u;
+                if (round < ROUNDS) { request(round, prv); }
+              }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+          }
+        } else {
 #pragma unroll
         for (int quadrant = 0; quadrant < 4; ++quadrant) {
           const int ha = quadrant / 2, hb = quadrant % 2;
@@ -751,13 +792,8 @@ __global__ __launch_bounds__(Config::THREADS, Config::MIN_WAVES) void LayerGemmK
             }
             __builtin_amdgcn_sched_barrier(0);
           }
-          if (quadrant == 1) {
-            // slab + 1 must have landed for everybody; the requests for the slabs behind it may stay in flight
-            constexpr int IN_FLIGHT = (LATER >= 2) ? (LATER - 1) * ROUNDS : 0;
-            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(IN_FLIGHT) : "memory");
-            if (LATER == 1) { zero_tail(nxt); }  // slab + 1 is the last one
-            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-          }
+          if (quadrant == 1) { next_slab_in_place(); }
+        }
         }
         cur = nxt;
         if (LOAD) {
@@ -766,16 +802,45 @@ __global__ __launch_bounds__(Config::THREADS, Config::MIN_WAVES) void LayerGemmK
         }
       };
       int slab = 0;
-      for (; slab + AHEAD < slabs; ++slab) { slab_body(std::integral_constant<int, AHEAD>{}); }
-      const auto last_slabs = [&](auto self, auto later_tag) {
-        constexpr int LATER = decltype(later_tag)::value;
-        if (slab + LATER < slabs) {
-          slab_body(later_tag);
-          ++slab;
+      using Even = std::integral_constant<int, 0>;
+      using Odd = std::integral_constant<int, WIDE ? 1 : 0>;
+      using Steady = std::integral_constant<int, AHEAD>;
+      using Last = std::integral_constant<int, AHEAD - 1>;
+      if constexpr (WIDE) {
+        // the last slabs, from the one that LATER others follow on; the sets of fragments take turns
+        const auto last_slabs = [&](auto self, auto later_tag, auto parity_tag) {
+          constexpr int LATER = decltype(later_tag)::value, PARITY = decltype(parity_tag)::value;
+          if (slab + LATER < slabs) {
+            slab_body(later_tag, parity_tag);
+            ++slab;
+            if constexpr (LATER > 0) { self(self, std::integral_constant<int, LATER - 1>{}, std::integral_constant<int, 1 - PARITY>{}); }
+          } else {
+            if constexpr (LATER > 0) { self(self, std::integral_constant<int, LATER - 1>{}, parity_tag); }
+          }
+        };
+        for (; slab + AHEAD + 1 < slabs; slab += 2) {
+          slab_body(Steady{}, Even{});
+          slab_body(Steady{}, Odd{});
         }
-        if constexpr (LATER > 0) { self(self, std::integral_constant<int, LATER - 1>{}); }
-      };
-      last_slabs(last_slabs, std::integral_constant<int, AHEAD - 1>{});
+        if (slab + AHEAD < slabs) {
+          slab_body(Steady{}, Even{});
+          ++slab;
+          last_slabs(last_slabs, Last{}, Odd{});
+        } else {
+          last_slabs(last_slabs, Last{}, Even{});
+        }
+      } else {
+        const auto last_slabs = [&](auto self, auto later_tag) {
+          constexpr int LATER = decltype(later_tag)::value;
+          if (slab + LATER < slabs) {
+            slab_body(later_tag, Even{});
+            ++slab;
+          }
+          if constexpr (LATER > 0) { self(self, std::integral_constant<int, LATER - 1>{}); }
+        };
+        for (; slab + AHEAD < slabs; ++slab) { slab_body(Steady{}, Even{}); }
+        last_slabs(last_slabs, Last{});
+      }
     };
     if (m0 + TILE_M <= p.m && n0 + TILE_N <= rows && k_tail == 0) { walk(std::false_type{}); }
     else { walk(std::true_type{}); }

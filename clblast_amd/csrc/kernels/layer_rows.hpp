@@ -69,8 +69,8 @@ __global__ __launch_bounds__(kLayerRowsThreads, UPSTREAM ? 5 : 4) void LayerRows
         const long long row = min(row0 + WAVES * u, end - 1);  // (a row beyond the chunk: the last one again, not used)
 #pragma unroll
         for (int e = 0; e < V; ++e) { z[u][e] = 0.0f; old[u][e] = 0.0f; }
-        if constexpr (UPSTREAM) { LayerPiece<T, V>::Load(static_cast<const T*>(q.upstream) + row * q.upstream_ld + col, inside, z[u]); }
-        if (other != nullptr) { LayerPiece<T, V>::Load(other + row * other_ld + col, inside, old[u]); }
+        if constexpr (UPSTREAM) { LayerPiece<T, V>::template Load<true>(static_cast<const T*>(q.upstream) + row * q.upstream_ld + col, inside, z[u]); }
+        if (other != nullptr) { LayerPiece<T, V>::template Load<UPSTREAM>(other + row * other_ld + col, inside, old[u]); }
       }
       if constexpr (!UPSTREAM) {
         const float* from = p.partials + static_cast<long long>(row0) * p.m + col;
