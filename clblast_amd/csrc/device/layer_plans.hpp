@@ -24,8 +24,8 @@ struct LayerTile {
   double alone_16, full_16, fixed_16, alone_32, full_32, fixed_32;
 };
 constexpr LayerTile kLayerTiles[] = {
-    {0, 128, 128, 2, 7.3, 8.6, 1.5, 61.6, 58.0, 2.0}, {1, 256, 256, 1, 17.0, 24.8, 8.0, 0.0, 0.0, 0.0},
-    {2, 256, 128, 2, 15.0, 14.9, 4.0, 0.0, 0.0, 0.0}, {3, 64, 64, 4, 4.1, 3.7, 0.2, 16.8, 14.6, 0.3},
+    {0, 128, 128, 2, 7.3, 9.3, 0.4, 61.6, 58.0, 2.0}, {1, 256, 256, 1, 17.0, 25.4, 4.5, 0.0, 0.0, 0.0},
+    {2, 256, 128, 2, 15.0, 15.2, 1.5, 0.0, 0.0, 0.0}, {3, 64, 64, 4, 4.1, 3.7, 0.2, 16.8, 14.6, 0.3},
     {4, 128, 32, 4, 0.0, 0.0, 0.0, 18.5, 16.0, 0.3},
 };
 constexpr int kLayerTileCount = sizeof(kLayerTiles) / sizeof(kLayerTiles[0]);
@@ -68,19 +68,19 @@ inline int LayerRowsChunk(const long long rows, const long long column_blocks) {
 
 inline int LayerVector(const int type) { return type == CLBH_TYPE_FP32 ? 4 : 8; }
 
-// Estimated time in us of `groups` work-groups of a tile that each walk k: rounds of as many as stay resident, the last one with
-// what is left. (256 x 4096 x 4096 in bf16 on 64 x 64 tiles: 35 estimated, 32 measured; 8192 x 8192 x 1024 on 256 x 256: 146 and
-// 137; 1024 x 1024 x 8192 in four ranges on 128 x 128: 37 and 39.)
+// Estimated time in us of so many work-groups of a tile that each walk k: rounds of as many as stay resident, the last one with
+// what is left; no round is over before its first loads and its stores have had their latencies. (bf16: 256 x 4096 x 4096 on
+// 64 x 64 22 estimated, 21 measured; 8192 x 8192 x 1024 on 256 x 256 125 and 121; 1024 x 4096 x 4096 on 128 x 128 35 and 40.)
 inline double LayerCost(const LayerTile& t, const bool wide, const double work_groups, const double k, const int units) {
   const double alone = (wide ? t.alone_32 : t.alone_16) * k * 1e-3, full = (wide ? t.full_32 : t.full_16) * k * 1e-3;
-  const double fixed = wide ? t.fixed_32 : t.fixed_16;
+  const double fixed = wide ? t.fixed_32 : t.fixed_16, latency = 2.5;
   const double slots = static_cast<double>(units) * t.per_cu;
   const double rounds = static_cast<double>(static_cast<long long>(work_groups / slots));
-  double cost = 5.0 + rounds * t.per_cu * (full + fixed);
+  double cost = 2.5 + rounds * std::max(t.per_cu * (full + fixed), alone + latency);
   const double left = (work_groups - rounds * slots) / units;  // work-groups per compute unit in the last round
   if (left > 0.0) {
     const double together = static_cast<double>(static_cast<long long>(left + 0.999));
-    cost += std::max(alone, (t.per_cu == 1 ? left : together) * full) + together * fixed;
+    cost += std::max((t.per_cu == 1 ? left : together) * full + together * fixed, alone + latency);
   }
   return cost;
 }
@@ -97,7 +97,9 @@ inline void ChooseLayerTile(const clbh_layer_desc& d, const int units, int& vari
     // (of groups the host knows the number alone: even ones are assumed)
     const double rows = by_rows ? static_cast<double>((d.n + d.groups - 1) / d.groups) : static_cast<double>(d.n);
     const double along_n = static_cast<double>(static_cast<long long>((rows + t.tile_n - 1) / t.tile_n)) * (by_rows ? std::min(d.groups, d.n) : 1);
-    const double groups = along_m * along_n * (by_depth ? d.groups : 1);
+    // (of groups by depth every XCD has an eighth of each group's tiles)
+    const double tiles = along_m * along_n;
+    const double groups = by_depth ? static_cast<double>(static_cast<long long>((tiles + 7.0) / 8.0)) * 8.0 * d.groups : tiles;
     const double k = by_depth ? std::max(1.0, static_cast<double>(d.k) / d.groups) : static_cast<double>(d.k);
     for (int s = 1; s <= 32; s = (s < 4) ? s + 1 : s + s / 2) {
       if (s > 1 && (d.grouping != CLBH_GROUPS_NONE || d.k < 256 * s)) { break; }

@@ -345,7 +345,8 @@ __device__ __forceinline__ GlobalBytes UniformAddress(const void* pointer) {
 
 // V consecutive values of a row, of which the first `inside` exist, as one access at whatever address the row starts (the
 // hardware splits one that is not aligned). Results are stored past the caches' keeping: they are not read again here and would push
-// out the operands that neighbouring tiles share (8192 x 8192 x 1024 142 -> 121 us, x 4096 with GELU and Z 476 -> 462 us).
+// out the operands that neighbouring tiles share (8192 x 8192 x 1024 142 -> 121 us, x 4096 with GELU and Z 476 -> 462 us);
+// so does a residual, read once (what it adds to the former: 45 -> 31 us).
 template <typename T, int V>
 struct LayerPiece {
   typedef T Piece __attribute__((ext_vector_type(V), aligned(sizeof(T))));
@@ -356,7 +357,7 @@ struct LayerPiece {
   }
   // at a uniform address and a lane's byte offset from there (the access carries both, no address is computed)
   typedef __attribute__((address_space(1))) Piece* GlobalPiece;
-  static __device__ __forceinline__ Raw LoadAt(const GlobalBytes base, const unsigned offset) { return *(GlobalPiece)(base + offset); }
+  static __device__ __forceinline__ Raw LoadAt(const GlobalBytes base, const unsigned offset) { return __builtin_nontemporal_load((GlobalPiece)(base + offset)); }
   static __device__ __forceinline__ void StoreAt(const GlobalBytes base, const unsigned offset, const float (&values)[V]) {
     Piece piece;
 #pragma unroll

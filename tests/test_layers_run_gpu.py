@@ -1,0 +1,313 @@
+"""The layer products as they are used: a feed-forward block and a block of experts trained through them, against automatic
+differentiation in 64 bits; recorded into a graph and replayed; on other streams than the current one; with offsets and strides
+beyond 32 bits; the same call again with the same bits."""
+import threading
+
+import pytest
+import torch
+
+import clblast_amd
+from clblast_amd import api
+from tests import layer_reference as ref
+
+pytestmark = pytest.mark.gpu
+
+TYPES = (torch.bfloat16, torch.float16, torch.float32)
+# A chain of products in the storage type: every tensor in between is rounded (half a step, 2^-8, 2^-11 or 2^-24 of a value),
+# and an error that enters a product of k random terms leaves it with the same size relative to the result's root mean
+# square. Four roundings at most lie between the inputs and a gradient here, and activations enlarge one by at most 1.13:
+# 4 * 1.13^2 * 2^-8 = 0.02 of the root mean square for a typical element; the bound is on the relative Frobenius norm, where
+# rounding errors are uniform in +- half a step (a factor of sqrt(1/3)): below 4 * 1.13^2 / sqrt(3) = 3 half steps.
+NORM = {torch.bfloat16: 3 * 2.0 ** -8, torch.float16: 3 * 2.0 ** -11, torch.float32: 3 * 2.0 ** -20}
+
+
+def generator(seed):
+    return torch.Generator(device="cuda:0").manual_seed(seed)
+
+
+def near(got, want, dtype, what):
+    error = float((got.double() - want).norm() / want.norm())
+    assert error <= NORM[dtype], (what, error)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("kind", ("gelu", "silu"))
+def test_training_step_of_a_feed_forward_block(gpu, dtype, kind):
+    """Y = X + act(X W1 + b1) W2^T + b2 and all of its gradients"""
+    g = generator(1)
+    tokens, width, hidden = 333, 264, 520
+    draw = lambda scale, *shape: (torch.randn(*shape, generator=g, device="cuda:0") * scale).to(dtype)
+    x, w1, b1 = draw(1, tokens, width), draw(width ** -0.5, width, hidden), draw(0.1, hidden)
+    w2, b2, dy = draw(hidden ** -0.5, width, hidden), draw(0.1, width), draw(1, tokens, width)
+    z, h, y = (torch.empty(tokens, n, dtype=dtype, device="cuda:0") for n in (hidden, hidden, width))
+    api.gemmEpilogue(None, tokens, hidden, width, x, w1, h, width, hidden, hidden, bias=b1, activation=kind, pre=z, pre_ld=hidden)
+    api.gemmEpilogue(None, tokens, width, hidden, h, w2, y, hidden, hidden, width, b_transp=True, bias=b2, beta=1.0, residual=x, residual_ld=width)
+    dz, db1, db2 = torch.empty_like(z), torch.empty_like(b1), torch.empty_like(b2)
+    dw1, dw2, dx = torch.empty_like(w1), torch.empty_like(w2), torch.empty_like(x)
+    api.activationGradient(None, tokens, width, dy, None, None, width, 0, 0, bias_gradient=db2)
+    api.gemmEpilogue(None, width, hidden, tokens, dy, h, dw2, width, hidden, hidden, a_transp=True)
+    api.gemmActivationGradient(None, tokens, hidden, width, dy, w2, z, dz, width, hidden, hidden, hidden, activation=kind, bias_gradient=db1)
+    api.gemmEpilogue(None, width, hidden, tokens, x, dz, dw1, width, hidden, hidden, a_transp=True)
+    api.gemmEpilogue(None, tokens, width, hidden, dz, w1, dx, hidden, hidden, width, b_transp=True, beta=1.0, residual=dy, residual_ld=width)
+    torch.cuda.synchronize()
+    leaves = [t.double().requires_grad_() for t in (x, w1, b1, w2, b2)]
+    X, W1, B1, W2, B2 = leaves
+    Y = X + ref.act(X @ W1 + B1, kind) @ W2.T + B2
+    Y.backward(dy.double())
+    near(y, Y.detach(), dtype, "y")
+    for name, got, leaf in zip(("dx", "dw1", "db1", "dw2", "db2"), (dx, dw1, db1, dw2, db2), leaves):
+        near(got, leaf.grad, dtype, name)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_training_step_of_a_block_of_experts(gpu, dtype):
+    """Y_g = silu(X_g W1_g + b1_g) W2_g^T for ragged groups, one of them empty, rows of nobody at the end, and its gradients"""
+    g = generator(2)
+    sizes, width, hidden = [40, 0, 131, 1, 77], 136, 200
+    groups, used, rows = len(sizes), sum(sizes), sum(sizes) + 7
+    offsets = torch.tensor([0] + sizes, device="cuda:0").cumsum(0)
+    draw = lambda scale, *shape: (torch.randn(*shape, generator=g, device="cuda:0") * scale).to(dtype)
+    x, w1, b1 = draw(1, rows, width), draw(width ** -0.5, groups, width, hidden), draw(0.1, groups, hidden)
+    w2, dy = draw(hidden ** -0.5, groups, width, hidden), draw(1, rows, width)
+    z, h, dh, dz = (torch.full((rows, hidden), 9.0, dtype=dtype, device="cuda:0") for _ in range(4))
+    y, dx = (torch.full((rows, width), 9.0, dtype=dtype, device="cuda:0") for _ in range(2))
+    dw1, dw2, db1 = torch.empty_like(w1), torch.empty_like(w2), torch.empty_like(b1)
+    each = width * hidden
+    api.gemmGrouped(None, groups, rows, hidden, width, x, w1, h, offsets, width, hidden, hidden, each, bias=b1, activation="silu", pre=z, pre_ld=hidden)
+    api.gemmGrouped(None, groups, rows, width, hidden, h, w2, y, offsets, hidden, hidden, width, each, b_transp=True)
+    api.gemmGroupedGradient(None, groups, rows, width, hidden, dy, h, dw2, offsets, width, hidden, hidden, each)
+    api.gemmGrouped(None, groups, rows, hidden, width, dy, w2, dh, offsets, width, hidden, hidden, each)
+    api.activationGradient(None, rows, hidden, dh, z, dz, hidden, hidden, hidden, activation="silu", bias_gradient=db1, group_count=groups, group_offsets=offsets)
+    api.gemmGroupedGradient(None, groups, rows, width, hidden, x, dz, dw1, offsets, width, hidden, hidden, each)
+    api.gemmGrouped(None, groups, rows, width, hidden, dz, w1, dx, offsets, hidden, hidden, width, each, b_transp=True)
+    torch.cuda.synchronize()
+    leaves = [t.double().requires_grad_() for t in (x, w1, b1, w2)]
+    X, W1, B1, W2 = leaves
+    at, parts = 0, []
+    for e, size in enumerate(sizes):
+        parts.append(ref.act(X[at:at + size] @ W1[e] + B1[e], "silu") @ W2[e].T)
+        at += size
+    Y = torch.cat(parts)
+    Y.backward(dy[:used].double())
+    near(y[:used], Y.detach(), dtype, "y")
+    near(dx[:used], X.grad[:used], dtype, "dx")
+    for name, got, leaf in zip(("dw1", "db1", "dw2"), (dw1, db1, dw2), (W1, B1, W2)):
+        near(got, leaf.grad, dtype, name)
+        assert bool((got[1] == 0).all()), "the empty expert's " + name
+    for t in (z, h, dh, dz, y, dx):
+        assert bool((t[used:] == 9.0).all()), "rows of nobody"
+
+
+def test_a_gradient_against_differences(gpu):
+    """The step's own directional derivative in fp32. The loss is a sum of 96 * 80 products of order one: its two values are off
+    by about sqrt(7680) * 2^-22 = 2e-5 (a few roundings of 2^-24 each), over 2h = 0.02 that is 1e-3; the third derivative adds
+    h^2 / 6 times a sum of 7680 terms of order one and of either sign, 1.7e-5 * 88 * 2 = 3e-3. The bound is twelve times
+    their sum; the derivative itself is of the order of sqrt(7680) = 88."""
+    g = generator(3)
+    m, n, k, h = 96, 80, 64, 0.01
+    draw = lambda *shape: torch.randn(*shape, generator=g, device="cuda:0")
+    x, w, b, direction, weight = draw(m, k), draw(k, n) * k ** -0.5, draw(n), draw(k, n) * k ** -0.5, draw(m, n)
+
+    def loss(matrix):
+        y = torch.empty(m, n, device="cuda:0")
+        api.gemmEpilogue(None, m, n, k, x, matrix.contiguous(), y, k, n, n, bias=b, activation="gelu")
+        return float((y.double() * weight.double()).sum())
+
+    z, dz, dw = torch.empty(m, n, device="cuda:0"), torch.empty(m, n, device="cuda:0"), torch.empty(k, n, device="cuda:0")
+    y = torch.empty(m, n, device="cuda:0")
+    api.gemmEpilogue(None, m, n, k, x, w, y, k, n, n, bias=b, activation="gelu", pre=z, pre_ld=n)
+    api.activationGradient(None, m, n, weight, z, dz, n, n, n, activation="gelu")
+    api.gemmEpilogue(None, k, n, m, x, dz, dw, k, n, n, a_transp=True)
+    slope = float((dw.double() * direction.double()).sum())
+    difference = (loss(w + h * direction) - loss(w - h * direction)) / (2 * h)
+    assert abs(slope - difference) <= 0.05, (slope, difference)
+
+
+def everything(t, stream=None):
+    """Calls of all five operators, with K ranges, copies of unaligned operands and sums in the workspace"""
+    m, n, k = 130, 264, 2048
+    api.gemmEpilogue(stream, m, n, k, t["a"], t["b"], t["c"], k, k, n, b_transp=True, bias=t["bias"], activation="gelu", pre=t["z"], pre_ld=n)
+    api.gemmEpilogue(stream, m, 71, 131, t["a"], t["b"], t["odd"], 131, 71, 71, activation="relu", a_offset=1, b_offset=3)
+    api.gemmActivationGradient(stream, m, n, k, t["a"], t["b"], t["z"], t["dz"], k, k, n, n, b_transp=True, activation="gelu", bias_gradient=t["db"])
+    api.activationGradient(stream, m, n, t["c"], t["z"], t["dz2"], n, n, n, activation="silu", bias_gradient=t["db2"], group_count=4, group_offsets=t["offsets"])
+    api.gemmGrouped(stream, 4, m, 64, n, t["c"], t["b"], t["y"], t["offsets"], n, 64, 64, n * 64, activation="silu")
+    api.gemmGroupedGradient(stream, 4, m, n, 64, t["c"], t["y"], t["dw"], t["offsets"], n, 64, 64, n * 64)
+
+
+OUTPUTS = ("c", "z", "odd", "dz", "db", "dz2", "db2", "y", "dw")
+
+
+def tensors(dtype, seed):
+    g = generator(seed)
+    m, n, k = 130, 264, 2048
+    draw = lambda *shape: torch.randn(*shape, generator=g, device="cuda:0").to(dtype)
+    t = {"a": draw(m * k + 8), "b": draw(n * k + 8), "bias": draw(n), "offsets": torch.tensor([0, 30, 30, 99, 125], device="cuda:0")}
+    for name, shape in zip(OUTPUTS, ((m, n), (m, n), (m, 71), (m, n), (n,), (m, n), (4, n), (m, 64), (4, n, 64))):
+        t[name] = torch.zeros(shape, dtype=dtype, device="cuda:0")
+    return t
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_the_same_call_gives_the_same_bits(gpu, dtype):
+    first, second = tensors(dtype, 4), tensors(dtype, 4)
+    for _ in range(3):
+        everything(first)
+        everything(second)
+        torch.cuda.synchronize()
+        for name in OUTPUTS:
+            assert torch.equal(first[name], second[name]), name
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_recorded_into_a_graph(gpu, dtype):
+    """Replays with other inputs and other groups against eager calls, with the program's own work in between"""
+    t, other = tensors(dtype, 5), tensors(dtype, 5)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        everything(t)  # un-captured: the stream's scratch buffer now exists
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        everything(t)
+    torch.cuda.synchronize()
+    for replay, offsets in enumerate(([0, 30, 30, 99, 125], [0, 0, 0, 0, 130], [5, 6, 70, 71, 71], [0, 130, 130, 130, 130])):
+        fresh = tensors(dtype, 10 + replay)
+        for both in (t, other):
+            for name in ("a", "b", "bias"):
+                both[name].copy_(fresh[name])
+            both["offsets"].copy_(torch.tensor(offsets, device="cuda:0"))
+            for name in OUTPUTS:
+                both[name].zero_()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        everything(other)
+        torch.cuda.synchronize()
+        for name in OUTPUTS:
+            assert torch.equal(t[name], other[name]), (replay, name)
+    assert clblast_amd.clear_cache() == 0
+
+
+def test_streams_and_threads(gpu):
+    """Four threads on streams of their own, two of them with the stream as an argument, against the same calls made alone"""
+    wanted = {}
+    for seed in range(4):
+        t = tensors(torch.bfloat16, 20 + seed)
+        everything(t)
+        torch.cuda.synchronize()
+        wanted[seed] = {name: t[name].clone() for name in OUTPUTS}
+    failures = []
+
+    def work(seed):
+        try:
+            stream = torch.cuda.Stream()
+            t = tensors(torch.bfloat16, 20 + seed)
+            torch.cuda.synchronize()
+            for _ in range(5):
+                if seed % 2:
+                    everything(t, stream)
+                else:
+                    with torch.cuda.stream(stream):
+                        everything(t)
+            stream.synchronize()
+            for name in OUTPUTS:
+                if not torch.equal(t[name], wanted[seed][name]):
+                    failures.append((seed, name))
+        except Exception as error:  # noqa: BLE001 - reported by the main thread
+            failures.append((seed, error))
+
+    threads = [threading.Thread(target=work, args=(seed,)) for seed in range(4)]
+    for thread in threads:
+        thread.start()
+    for thread in threads:
+        thread.join()
+    assert not failures, failures
+
+
+def test_offsets_and_strides_beyond_32_bits(gpu):
+    """Rows of C, of Z and of the residual 2^31 elements apart, an operand with lines further apart than the tiled kernel
+    reaches, experts more than 2^32 bytes apart"""
+    dtype, m, n, k = torch.bfloat16, 3, 72, 64
+    g = generator(6)
+    draw = lambda *shape: torch.randn(*shape, generator=g, device="cuda:0").to(dtype)
+    far = (1 << 31) + 10
+    big = torch.zeros(2 * far + n + 8, dtype=dtype, device="cuda:0")  # 8.6 GB
+    a, b = draw(m, k), draw(n, k)
+    residual = draw(m, n)
+    rows = big.as_strided((m, n), (far, 1))
+    rows.copy_(residual)
+    want, bound, want_z, z_bound = ref.epilogue(a.double(), b.double().T, dtype, 1.0, None, "gelu", 1.0, residual.double())
+    z = torch.zeros(m, n, dtype=dtype, device="cuda:0")
+    api.gemmEpilogue(None, m, n, k, a, b, big, k, k, far, b_transp=True, activation="gelu", pre=z, pre_ld=n, beta=1.0, residual=big, residual_ld=far)
+    torch.cuda.synchronize()
+    ref.check(rows, want, bound, "rows of C far apart")
+    ref.check(z, want_z, z_bound, "z")
+    assert float(big[n:n + 4096].abs().max()) == 0.0 and float(big[far - 4096:far].abs().max()) == 0.0
+    lines = (1 << 21) + 5
+    rows_of_a = big[:].as_strided((m, k), (lines, 1))
+    rows_of_a.copy_(a)
+    c = torch.zeros(m, n, dtype=dtype, device="cuda:0")
+    api.gemmEpilogue(None, m, n, k, big, b, c, lines, k, n, b_transp=True, activation="gelu")
+    want, bound, _, _ = ref.epilogue(a.double(), b.double().T, dtype, kind="gelu")
+    torch.cuda.synchronize()
+    ref.check(c, want, bound, "lines of A far apart")
+    experts = big.as_strided((2, n, k), (far, k, 1))
+    weights = draw(2, n, k)
+    experts.copy_(weights)
+    offsets = torch.tensor([0, 1, 3], device="cuda:0")
+    api.gemmGrouped(None, 2, m, n, k, a, big, c, offsets, k, k, n, far, b_transp=True)
+    torch.cuda.synchronize()
+    for e, (begin, end) in enumerate(((0, 1), (1, 3))):
+        want, bound, _, _ = ref.epilogue(a[begin:end].double(), weights[e].double().T, dtype)
+        ref.check(c[begin:end], want, bound, "expert %d" % e)
+    result = big.as_strided((2, k, n), (far, n, 1))
+    api.gemmGroupedGradient(None, 2, m, k, n, a, c, big, offsets, k, n, n, far)
+    torch.cuda.synchronize()
+    for e, (begin, end) in enumerate(((0, 1), (1, 3))):
+        want, bound, _, _ = ref.epilogue(a[begin:end].double().T, c[begin:end].double(), dtype)
+        ref.check(result[e], want, bound, "gradient of expert %d" % e)
+
+
+def test_special_values(gpu):
+    """Infinities and NaN stay in their rows and columns; a residual with beta = 0, rows of nobody and padding bring none in
+    (the other tests fill those with NaN); large finite inputs of the activations give finite slopes"""
+    for dtype in TYPES:
+        g = generator(7)
+        m, n, k = 70, 72, 40
+        a, b = torch.randn(m, k, generator=g, device="cuda:0").to(dtype), torch.randn(k, n, generator=g, device="cuda:0").to(dtype)
+        a[3, 5], a[9, 0] = float("nan"), float("inf")
+        c = torch.zeros(m, n, dtype=dtype, device="cuda:0")
+        api.gemmEpilogue(None, m, n, k, a, b, c, k, n, n)
+        torch.cuda.synchronize()
+        assert bool(c[3].isnan().all()) and bool((~c[9].isfinite()).all())
+        rest = torch.ones(m, dtype=torch.bool, device="cuda:0")
+        rest[3] = rest[9] = False
+        assert bool(c[rest].isfinite().all())
+        largest = torch.finfo(dtype).max
+        z = torch.tensor([[-largest, largest, -200.0, 200.0, -1e4, 1e4, 0.0, -0.0]], device="cuda:0").to(dtype)
+        one = torch.ones_like(z)
+        for kind, ends in (("relu", (0, 1)), ("gelu", (0, 1)), ("gelu_tanh", (0, 1)), ("silu", (0, 1)), ("none", (1, 1))):
+            out = torch.zeros_like(z)
+            api.activationGradient(None, 1, 8, one, z, out, 8, 8, 8, activation=kind)
+            torch.cuda.synchronize()
+            expected = [ends[0], ends[1]] * 3
+            assert [float(v) for v in out[0, :6]] == expected, (dtype, kind, out)
+
+
+def test_python_calls_on_other_devices_and_types(gpu):
+    a = torch.zeros(8, 8, dtype=torch.float64, device="cuda:0")
+    with pytest.raises(ValueError, match="data-type"):
+        api.gemmEpilogue(None, 8, 8, 8, a, a, a, 8, 8, 8)
+    a = a.half()
+    with pytest.raises(ValueError, match="one GPU"):
+        api.gemmEpilogue(None, 8, 8, 8, a, a.cpu(), a, 8, 8, 8)
+    offsets = torch.tensor([0, 8], dtype=torch.int32, device="cuda:0")
+    with pytest.raises(ValueError, match="64-bit"):
+        api.gemmGrouped(None, 1, 8, 8, 8, a, a, a, offsets, 8, 8, 8, 64)
+    with pytest.raises(clblast_amd.CLBlastError) as error:
+        api.gemmGrouped(None, 0, 8, 8, 8, a, a, a, offsets.long(), 8, 8, 8, 64)
+    assert error.value.status == -2049
+    with pytest.raises(clblast_amd.CLBlastError) as error:
+        api.gemmEpilogue(None, 8, 8, 8, a, a, a, 7, 8, 8)
+    assert error.value.status == -1016
