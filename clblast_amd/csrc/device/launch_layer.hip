@@ -18,6 +18,7 @@ bool ValidLayer(const clbh_layer_desc& d) {
     return reinterpret_cast<unsigned long long>(pointer) % (d.type == CLBH_TYPE_FP32 ? 4 : 2) == 0;
   };
   if (d.type != CLBH_TYPE_FP16 && d.type != CLBH_TYPE_BF16 && d.type != CLBH_TYPE_FP32) { return false; }
+  if (d.m > CLBH_LAYER_MAX_SIZE || d.n > CLBH_LAYER_MAX_SIZE || d.k > CLBH_LAYER_MAX_SIZE) { return false; }
   if (d.m <= 0 || d.n <= 0 || d.activation < 161 || d.activation > 165) { return false; }
   if (d.grouping != CLBH_GROUPS_NONE) {
     if (d.offsets == nullptr || reinterpret_cast<unsigned long long>(d.offsets) % 8 != 0 || d.groups <= 0 || d.groups > CLBH_LAYER_MAX_GROUPS) { return false; }

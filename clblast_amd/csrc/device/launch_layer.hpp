@@ -142,10 +142,11 @@ int AlignLayerOperands(const clbh_layer_desc& d, const LayerPlan& plan, LayerArg
   const bool by_rows = d.grouping == CLBH_GROUPS_BY_ROWS;
   if (plan.a_copy_ld > 0) {
     const int lines = d.a_kcontig ? d.m : d.k;
-    describe(0, d.a, d.a_ld, by_rows ? d.a_stride : 0, plan.a_copy_ld, plan.a_copy_offset, d.a_kcontig ? d.k : d.m, lines, by_rows ? d.groups : 1);
+    describe(0, d.a, d.a_ld, by_rows ? d.a_stride : 0, plan.a_copy_ld, plan.a_copy_offset, d.a_kcontig ? d.k : d.m, lines,
+             (by_rows && d.a_stride != 0) ? d.groups : 1);
     args.a = q.operand[0].to;
     args.a_ld = plan.a_copy_ld;
-    args.a_stride = plan.a_copy_ld * lines;
+    args.a_stride = (d.a_stride != 0) ? plan.a_copy_ld * lines : 0;
   }
   if (plan.b_copy_ld > 0) {
     describe(1, d.b, d.b_ld, 0, plan.b_copy_ld, plan.b_copy_offset, d.b_kcontig ? d.k : d.n, d.b_kcontig ? d.n : d.k, 1);

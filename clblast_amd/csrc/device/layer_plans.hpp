@@ -150,7 +150,7 @@ inline LayerPlan PlanLayer(const clbh_layer_desc& d, const int units) {
     const bool by_rows = d.grouping == CLBH_GROUPS_BY_ROWS;
     if (!LayerOperandFits(d.a, d.a_ld, by_rows ? d.a_stride : 0, d.type)) {
       plan.a_copy_ld = ((d.a_kcontig ? d.k : d.m) + 7ll) / 8 * 8;
-      plan.a_copy_offset = take(size * static_cast<size_t>(plan.a_copy_ld) * static_cast<size_t>(d.a_kcontig ? d.m : d.k) * static_cast<size_t>(by_rows ? d.groups : 1));
+      plan.a_copy_offset = take(size * static_cast<size_t>(plan.a_copy_ld) * static_cast<size_t>(d.a_kcontig ? d.m : d.k) * static_cast<size_t>((by_rows && d.a_stride != 0) ? d.groups : 1));
     }
     if (!LayerOperandFits(d.b, d.b_ld, 0, d.type)) {
       plan.b_copy_ld = ((d.b_kcontig ? d.k : d.n) + 7ll) / 8 * 8;

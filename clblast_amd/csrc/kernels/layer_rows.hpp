@@ -180,7 +180,7 @@ __global__ __launch_bounds__(kLayerRowsThreads) void LayerColumnSumsKernel(const
         const long long from = offsets[g], to = offsets[g + 1];
         const int begin = static_cast<int>(from < 0 ? 0 : (from > rows ? rows : from));
         const int size = static_cast<int>(to < begin ? 0 : (to > rows ? rows : to) - begin);
-        before += (size + tile - 1) / tile;
+        before = min(before + (size + tile - 1) / tile, rows_of_sums);  // (groups that overlap can have any number of tiles)
       }
 #pragma unroll
       for (int step = 32; step >= 1; step /= 2) { before += __shfl_xor(before, step, 64); }

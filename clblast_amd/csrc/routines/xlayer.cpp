@@ -3,7 +3,6 @@
 // =================================================================================================
 #include "routines/xlayer.hpp"
 
-#include <climits>
 #include <memory>
 
 namespace clblast {
@@ -16,9 +15,9 @@ template <> constexpr int LayerType<bfloat16>() { return CLBH_TYPE_BF16; }
 template <> constexpr int LayerType<float>() { return CLBH_TYPE_FP32; }
 
 void TestSizes(const size_t m, const size_t n, const size_t k) {
-  constexpr auto kLimit = static_cast<size_t>(INT_MAX);
+  constexpr auto kLimit = static_cast<size_t>(CLBH_LAYER_MAX_SIZE);
   if (m == 0 || n == 0 || k == 0) { throw BLASError(StatusCode::kInvalidDimension); }
-  if (m > kLimit || n > kLimit || k > kLimit) { throw BLASError(StatusCode::kInvalidDimension, "dimension exceeds 2^31-1"); }
+  if (m > kLimit || n > kLimit || k > kLimit) { throw BLASError(StatusCode::kInvalidDimension, "dimension exceeds 2^31 - 1024"); }
 }
 
 void TestActivation(const Activation activation) {
@@ -243,7 +242,12 @@ void Xlayer<T>::DoGemmGroupedGradient(const size_t m, const size_t n, const size
   TestSizes(m, n, k);
   TestA(k, m, a, sizeof(T));
   TestB(k, n, b, sizeof(T));
-  if (c.ld >= n && groups.count > 1 && c_stride / c.ld < m) { throw BLASError(StatusCode::kInvalidLeadDimC, "results of the groups overlap"); }
+  if (c.ld >= n && groups.count > 1) {  // one behind the other, or side by side within the rows
+    using Wide = unsigned __int128;
+    const bool behind = c_stride >= static_cast<Wide>(m - 1) * c.ld + n;
+    const bool beside = c_stride >= n && static_cast<Wide>(groups.count - 1) * c_stride + n <= c.ld;
+    if (!behind && !beside) { throw BLASError(StatusCode::kInvalidLeadDimC, "results of the groups overlap"); }
+  }
   TestC(m, n, c, sizeof(T), groups.count, c_stride);
   TestOffsets(groups);
   auto desc = Describe<T>(m, n, k, alpha, Activation::kNone);

@@ -279,7 +279,8 @@ CLBH_API int clbh_conv_slab(int precision, const clbh_im2col_shape* shape, int k
 #define CLBH_GROUPS_BY_DEPTH 2
 #define CLBH_LAYER_MAX_LD (1ll << 23)        // operands: 16 lines of a slab stay at 32-bit byte offsets
 #define CLBH_LAYER_MAX_GROUPED (1ll << 26)   // rows (depths) of a grouped call
-#define CLBH_LAYER_MAX_GROUPS (1ll << 20)
+#define CLBH_LAYER_MAX_GROUPS (1ll << 16)    // every work-group looks through all of them
+#define CLBH_LAYER_MAX_SIZE ((1ll << 31) - 1024)  // m, n, k: a tile that begins inside ends below 2^31
 typedef struct clbh_layer_desc_ {
   int type;          // CLBH_TYPE_...
   int tile_variant;  // index into kLayerTiles (device/layer_plans.hpp), -1: chosen by size

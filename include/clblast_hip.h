@@ -240,7 +240,8 @@ StatusCode Convgemm(const KernelMode kernel_mode, const size_t channels, const s
 // matrices are row-major (a column-major caller exchanges A and B, and m and n); offsets, leading dimensions and strides
 // are in elements. The reference has no such routines. Zero sizes return kInvalidDimension, a group count of zero kInvalidBatchCount;
 // the codes of `pre` and `residual` are those of matrix C, the codes of `bias` and `bias_gradient` those of vector X, the
-// codes of `group_offsets` those of vector Y.
+// codes of `group_offsets` those of vector Y. Sizes are at most 2^31 - 1024, groups at most 65536. What is written overlaps
+// neither other results nor operands, but for the places that say so.
 
 // Z = alpha * op(A) * op(B) + bias, C = act(Z) + beta * R, for op(A) m x k, op(B) k x n and a bias of n values that every row
 // gets (nullptr: none). Z (m x n) is stored at `pre` as well unless that is nullptr; activation kNone makes this a
@@ -266,7 +267,7 @@ StatusCode GemmActivationGradient(const Transpose a_transpose, const Transpose b
                                   void* bias_gradient_buffer, const size_t bias_gradient_offset, hipStream_t* queue,
                                   hipEvent_t* event = nullptr);
 
-// The same where the gradient comes from elsewhere: C = Y . act'(Z) for m x n matrices, C may be Y itself. C may be nullptr
+// The same where the gradient comes from elsewhere: C = Y . act'(Z) for m x n matrices, C may be Y or Z itself. C may be nullptr
 // where only the sums are wanted. With groups (group_offsets not nullptr, see GemmGrouped) only their rows take part, and
 // bias_gradient holds group_count vectors of n values, one behind the other (zeros for a group without rows).
 template <typename T>

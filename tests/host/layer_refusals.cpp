@@ -116,6 +116,11 @@ int main() {
   epilogue(StatusCode::kInvalidDimension, "n = 0", A, B, V, P, 0.0f, nothing, C, 10, 0);
   epilogue(StatusCode::kInvalidDimension, "k = 0", A, B, V, P, 0.0f, nothing, C, 10, 12, 0);
   epilogue(StatusCode::kInvalidDimension, "m too large", A, B, V, P, 0.0f, nothing, C, size_t{1} << 32);
+  for (const auto size : {size_t{0x7fffffff}, (size_t{1} << 31) - 1023}) {  // a tile that begins inside would end beyond 32 bits
+    epilogue(StatusCode::kInvalidDimension, "m close to 2^31", A, B, V, P, 0.0f, nothing, C, size);
+    epilogue(StatusCode::kInvalidDimension, "n close to 2^31", A, B, V, P, 0.0f, nothing, C, 10, size);
+    epilogue(StatusCode::kInvalidDimension, "k close to 2^31", A, B, V, P, 0.0f, nothing, C, 10, 12, size);
+  }
   epilogue(StatusCode::kInvalidValue, "activation", A, B, V, P, 0.0f, nothing, C, 10, 12, 14, no, static_cast<Activation>(7));
   epilogue(StatusCode::kInvalidValue, "transpose", A, B, V, P, 0.0f, nothing, C, 10, 12, 14, static_cast<Transpose>(1));
   epilogue(StatusCode::kInvalidLeadDimA, "a_ld", LayerMatrix{a, 0, 13}, B, V, P, 0.0f, nothing, C);
@@ -173,7 +178,7 @@ int main() {
   grouped(StatusCode::kInsufficientMemoryB, "experts short", 14 * 12 + 1, none, three);
   grouped(StatusCode::kInsufficientMemoryB, "stride overflows", ~size_t{0} / 2, none, three);
   grouped(StatusCode::kInvalidIncrementX, "biases overlap", 14 * 12, LayerVector{sums, 0, 11}, three);
-  grouped(StatusCode::kInvalidBatchCount, "too many groups", 0, none, LayerGroups{(size_t{1} << 20) + 1, offsets, 0});
+  grouped(StatusCode::kInvalidBatchCount, "too many groups", 0, none, LayerGroups{(size_t{1} << 16) + 1, offsets, 0});
   grouped(StatusCode::kInvalidVectorY, "no offsets", 0, none, LayerGroups{3, nullptr, 0});
   grouped(StatusCode::kInvalidDimension, "no rows", 0, none, three, 0);
 
@@ -182,6 +187,12 @@ int main() {
   };
   depth(StatusCode::kSuccess, "grouped gradient", 12, 14 * 12);
   depth(StatusCode::kInvalidLeadDimC, "results overlap", 12, 13 * 12);
+  depth(StatusCode::kInvalidLeadDimC, "results overlap by an element", 13, 13 * 13 + 11);
+  depth(StatusCode::kSuccess, "results without the last row's padding", 12, 13 * 12 + 12);
+  depth(StatusCode::kSuccess, "results side by side", 36, 12);
+  depth(StatusCode::kInvalidLeadDimC, "results side by side overlap", 36, 11);
+  depth(StatusCode::kInvalidLeadDimC, "results side by side reach the next row", 35, 12);
+  depth(StatusCode::kInvalidLeadDimC, "stride of zero", 36, 0);
   depth(StatusCode::kInvalidLeadDimC, "c_ld", 11, 14 * 12);
   depth(StatusCode::kInsufficientMemoryC, "results short", 12, 14 * 12 + 1);
   depth(StatusCode::kInvalidDimension, "no depth", 12, 14 * 12, 0);

@@ -311,3 +311,104 @@ def test_python_calls_on_other_devices_and_types(gpu):
     with pytest.raises(clblast_amd.CLBlastError) as error:
         api.gemmEpilogue(None, 8, 8, 8, a, a, a, 7, 8, 8)
     assert error.value.status == -1016
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_lines_of_an_operand_beyond_the_tiled_kernels_reach(gpu, dtype):
+    """Either operand with lines 2^23 and more elements apart, as it is and transposed"""
+    g = generator(30)
+    m, n, k = 37, 72, 24
+    draw = lambda *shape: torch.randn(*shape, generator=g, device="cuda:0").to(dtype)
+    for ld in ((1 << 23) - 2, 1 << 23, (1 << 23) + 6):
+        big = torch.full((37 * ld + 64,), float("nan"), dtype=dtype, device="cuda:0")
+        for transposed in (False, True):
+            a, b = draw(m, k), draw(k, n)
+            want, bound, _, _ = ref.epilogue(a.double(), b.double(), dtype)
+            far = big.as_strided((k, m) if transposed else (m, k), (ld, 1))
+            far.copy_(a.T if transposed else a)
+            c = torch.zeros(m, n, dtype=dtype, device="cuda:0")
+            api.gemmEpilogue(None, m, n, k, big, b, c, ld, n, n, a_transp=transposed)
+            torch.cuda.synchronize()
+            ref.check(c, want, bound, "a, %d apart" % ld)
+            # the other operand: its first 37 columns (rows) alone, so that the same memory does
+            far = big.as_strided((37, k) if transposed else (k, 37), (ld, 1))
+            far.copy_(b[:, :37].T if transposed else b[:, :37])
+            c = torch.zeros(m, 37, dtype=dtype, device="cuda:0")
+            api.gemmEpilogue(None, m, 37, k, a, big, c, k, ld, 37, b_transp=transposed)
+            torch.cuda.synchronize()
+            ref.check(c, want[:, :37], bound[:, :37], "b, %d apart" % ld)
+
+
+def test_sums_of_many_overlapping_groups(gpu):
+    """Offsets that go back and forth make every other group as long as the whole matrix: together the groups have far more
+    chunks of rows than there are (2^31 and more). What the sums hold then is not specified; nothing around them is touched, and
+    groups in order give the right sums right behind such a call."""
+    rows, groups = 1 << 25, 1 << 14
+    y = torch.ones(rows, 1, dtype=torch.float16, device="cuda:0")
+    sums = torch.full((groups + 128,), 7.0, dtype=torch.float16, device="cuda:0")
+    offsets = torch.zeros(groups + 1, dtype=torch.int64, device="cuda:0")
+    offsets[1::2] = rows
+    api.activationGradient(None, rows, 1, y, None, None, 1, 0, 0, bias_gradient=sums, group_count=groups, group_offsets=offsets, bias_gradient_offset=64)
+    torch.cuda.synchronize()
+    assert bool((sums[:64] == 7.0).all()) and bool((sums[groups + 64:] == 7.0).all())
+    offsets = torch.arange(groups + 1, device="cuda:0") * (rows // groups)
+    api.activationGradient(None, rows, 1, y, None, None, 1, 0, 0, bias_gradient=sums, group_count=groups, group_offsets=offsets, bias_gradient_offset=64)
+    torch.cuda.synchronize()
+    assert bool((sums[64:groups + 64] == rows // groups).all())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_results_of_groups_side_by_side(gpu, dtype):
+    """The groups' results as columns of one matrix, in place"""
+    g = generator(31)
+    sizes, m, n = [9, 0, 70], 40, 72
+    k, groups = sum(sizes), len(sizes)
+    draw = lambda *shape: torch.randn(*shape, generator=g, device="cuda:0").to(dtype)
+    a, b, c = draw(k, m), draw(k, n), draw(m, groups * n + 5)
+    old = c.clone()
+    offsets = torch.tensor([0] + sizes, device="cuda:0").cumsum(0)
+    api.gemmGroupedGradient(None, groups, k, m, n, a, b, c, offsets, m, n, groups * n + 5, n, beta=1.0)
+    torch.cuda.synchronize()
+    at = 0
+    for e, size in enumerate(sizes):
+        columns = slice(e * n, (e + 1) * n)
+        want, bound, _, _ = ref.epilogue(a[at:at + size].double().T, b[at:at + size].double(), dtype, 1.0, None, "none", 1.0, old[:, columns].double())
+        ref.check(c[:, columns], want, bound, "group %d" % e)
+        at += size
+    assert torch.equal(c[:, groups * n:], old[:, groups * n:])
+
+
+def test_two_graphs_of_one_stream(gpu):
+    """Two graphs captured on a stream share its scratch: replayed on it in turn, with eager calls in between"""
+    dtype = torch.bfloat16
+    first, second, other = (tensors(dtype, seed) for seed in (40, 41, 42))
+    wanted = []
+    for seed in (40, 41, 42):
+        t = tensors(dtype, seed)
+        everything(t)
+        torch.cuda.synchronize()
+        wanted.append({name: t[name].clone() for name in OUTPUTS})
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        everything(other)
+    side.synchronize()
+    graphs = []
+    for t in (first, second):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1], stream=side):
+            everything(t)
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for t in (first, second, other):
+            for name in OUTPUTS:
+                t[name].zero_()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            graphs[0].replay()
+            graphs[1].replay()
+            everything(other)
+        side.synchronize()
+        for t, want in zip((first, second, other), wanted):
+            for name in OUTPUTS:
+                assert torch.equal(t[name], want[name]), name
