@@ -112,10 +112,12 @@ int LaunchLayerRowsOf(const clbh_layer_desc& d, const LayerPlan& plan, const Lay
   q.upstream_ld = d.upstream_ld;
   q.ranges = (d.upstream != nullptr) ? 1 : plan.splits;
   q.chunk = plan.rows_chunk;
+  q.lane_shift = plan.rows_lane_shift;
   const long long column_blocks = (static_cast<long long>(d.m) + 64 * V - 1) / (64 * V);
   if (column_blocks * plan.rows_chunks > INT_MAX) { return hipErrorInvalidConfiguration; }
   q.column_blocks = static_cast<int>(column_blocks);
-  LayerRowsKernel<T, V, UPSTREAM><<<dim3(static_cast<unsigned>(column_blocks * plan.rows_chunks)), dim3(kLayerRowsThreads), 0, stream>>>(q);
+  const auto kernel = (plan.rows_lane_shift < 6) ? LayerRowsKernel<T, V, UPSTREAM, true> : LayerRowsKernel<T, V, UPSTREAM, false>;
+  kernel<<<dim3(static_cast<unsigned>(column_blocks * plan.rows_chunks)), dim3(kLayerRowsThreads), 0, stream>>>(q);
   return static_cast<int>(hipGetLastError());
 }
 
@@ -179,7 +181,9 @@ int LaunchLayerTyped(const clbh_layer_desc& d, const LayerPlan& plan, hipStream_
     const bool grouped = d.grouping == CLBH_GROUPS_BY_ROWS;
     const int groups = grouped ? d.groups : 1;
     const dim3 grid(static_cast<unsigned>((static_cast<long long>(d.m) + 63) / 64), static_cast<unsigned>(groups < 65535 ? groups : 65535));
-    LayerColumnSumsKernel<T><<<grid, dim3(kLayerRowsThreads), 0, stream>>>(
+    const bool many = rows_of_sums >= 64ll * groups;  // sums per group
+    const auto kernel = many ? LayerColumnSumsKernel<T, 16> : LayerColumnSumsKernel<T, 4>;
+    kernel<<<grid, dim3(many ? 1024 : 256), 0, stream>>>(
         args.bias_partials, static_cast<int>(rows_of_sums), d.m, grouped ? d.offsets : nullptr, groups, d.n,
         elementwise ? plan.rows_chunk : plan.tile.tile_n, static_cast<T*>(d.bias_gradient), static_cast<long long>(d.m));
     return static_cast<int>(hipGetLastError());

@@ -34,6 +34,7 @@ struct LayerPlan {
   LayerTile tile;
   long long tiles_m, tiles_n;  // tiles_n: for groups by rows the most there can be
   int splits, chunk;           // K ranges (1: none)
+  int rows_lane_shift;         // elementwise kernel: 2^ of it lanes per row
   int rows_chunk;              // rows per work-group of the elementwise kernel
   long long rows_chunks;       // work-groups of it along the rows (the most there can be)
   // operands that the kernel cannot fetch as they are and that are copied first (0: not), with the copy's leading dimension
@@ -59,11 +60,18 @@ inline bool LayerTileExists(const int type, const LayerTile& tile) {
 }
 
 // Rows per work-group of the elementwise kernel: as few as give about 2048 work-groups, at least 8 (two per wavefront), at
-// most 128
-inline int LayerRowsChunk(const long long rows, const long long column_blocks) {
-  int chunk = 8;
-  while (chunk < 128 && rows * column_blocks > 2048ll * chunk) { chunk *= 2; }
+// most 128, times the rows that a wavefront takes side by side
+inline int LayerRowsChunk(const long long rows, const long long column_blocks, const int lane_shift) {
+  int chunk = 8 * (64 >> lane_shift);
+  const int most = 16 * chunk;
+  while (chunk < most && rows * column_blocks > 2048ll * chunk) { chunk *= 2; }
   return chunk;
+}
+// A row of a narrow matrix is the work of 2^shift lanes, a wavefront takes 64 of them side by side
+inline int LayerRowsLaneShift(const long long features, const int vector) {
+  int shift = 0;
+  while (shift < 6 && (static_cast<long long>(vector) << shift) < features) { ++shift; }
+  return shift;
 }
 
 inline int LayerVector(const int type) { return type == CLBH_TYPE_FP32 ? 4 : 8; }
@@ -138,8 +146,10 @@ inline LayerPlan PlanLayer(const clbh_layer_desc& d, const int units) {
       }
     }
   }
-  const long long per_block = 64ll * ((d.upstream != nullptr) ? LayerVector(d.type) : 4), column_blocks = (d.m + per_block - 1) / per_block;
-  plan.rows_chunk = LayerRowsChunk(d.n, column_blocks);
+  const int vector = (d.upstream != nullptr) ? LayerVector(d.type) : 4;
+  const long long per_block = 64ll * vector, column_blocks = (d.m + per_block - 1) / per_block;
+  plan.rows_lane_shift = LayerRowsLaneShift(d.m, vector);
+  plan.rows_chunk = LayerRowsChunk(d.n, column_blocks, plan.rows_lane_shift);
   plan.rows_chunks = (d.grouping == CLBH_GROUPS_BY_ROWS) ? MostGroupTiles(d.n, d.groups, plan.rows_chunk) : (d.n + plan.rows_chunk - 1) / plan.rows_chunk;
   if (d.bias_gradient != nullptr) {
     const long long rows_of_sums = (d.upstream != nullptr || plan.splits > 1) ? plan.rows_chunks : plan.tiles_n;

@@ -22,13 +22,15 @@ struct LayerRowsArgs {
   long long upstream_ld;
   int ranges;            // K ranges at layer.partials
   int chunk;             // rows per work-group
+  int lane_shift;        // 2^lane_shift lanes per row, a wavefront takes 64 >> lane_shift rows side by side
   int column_blocks;     // work-groups side by side; the grid's only dimension counts them first
 };
 
-// Work-group: 64 pieces of V features (lanes) times `chunk` rows, which its four wavefronts take in turn. bias_partials: one
-// row of m sums for every chunk, the chunks numbered through the groups. UPSTREAM: the caller's matrix takes the place
-// of the sums.
-template <typename T, int V, bool UPSTREAM>
+// Work-group: 64 pieces of V features (lanes; fewer of a narrow matrix, several rows side by side then) times `chunk` rows, which its
+// four wavefronts take in turn. bias_partials: one row of m sums for every chunk, the chunks numbered through the groups. UPSTREAM: the caller's matrix takes the place
+// of the sums. NARROW: a row is the work of less than 64 lanes (65536 x 64 with all lanes on one row: 28 us, 9 like this;
+// 8192 x 8192 with row numbers in vector registers: 87 us, 74 with scalar ones).
+template <typename T, int V, bool UPSTREAM, bool NARROW>
 __global__ __launch_bounds__(kLayerRowsThreads, UPSTREAM ? 5 : 4) void LayerRowsKernel(const LayerRowsArgs q) {
   constexpr bool FAST = sizeof(T) == 2;
   constexpr int WAVES = kLayerRowsThreads / 64, FLIGHT = UPSTREAM ? 2 : 1;  // rows of a wavefront in flight together
@@ -37,7 +39,9 @@ __global__ __launch_bounds__(kLayerRowsThreads, UPSTREAM ? 5 : 4) void LayerRows
   __shared__ float wave_sums[WAVES][64 * V];
   const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const int column_block = blockIdx.x % q.column_blocks;
-  const int col = (column_block * 64 + lane) * V;
+  const int lane_shift = NARROW ? q.lane_shift : 6;
+  const int lanes = 1 << lane_shift, beside = 64 >> lane_shift;  // (less than 64 lanes: one column block)
+  const int col = (column_block * 64 + (lane & (lanes - 1))) * V;
   const int inside = p.m - col;  // features from this lane's first one on
 
   const int sums_row = blockIdx.x / q.column_blocks;
@@ -62,11 +66,11 @@ __global__ __launch_bounds__(kLayerRowsThreads, UPSTREAM ? 5 : 4) void LayerRows
   const long long other_ld = p.gradient ? p.pre_ld : p.residual_ld;
 
   if (inside > 0) {
-    for (int row0 = first + wave; row0 < end; row0 += WAVES * FLIGHT) {
+    for (int row0 = first + wave * beside + (NARROW ? lane >> lane_shift : 0); row0 < end; row0 += WAVES * FLIGHT * beside) {
       float z[FLIGHT][V], old[FLIGHT][V];
 #pragma unroll
       for (int u = 0; u < FLIGHT; ++u) {
-        const long long row = min(row0 + WAVES * u, end - 1);  // (a row beyond the chunk: the last one again, not used)
+        const long long row = min(row0 + WAVES * beside * u, end - 1);  // (a row beyond the chunk: the last one again, not used)
 #pragma unroll
         for (int e = 0; e < V; ++e) { z[u][e] = 0.0f; old[u][e] = 0.0f; }
         if constexpr (UPSTREAM) { LayerPiece<T, V>::template Load<true>(static_cast<const T*>(q.upstream) + row * q.upstream_ld + col, inside, z[u]); }
@@ -92,7 +96,7 @@ __global__ __launch_bounds__(kLayerRowsThreads, UPSTREAM ? 5 : 4) void LayerRows
       }
 #pragma unroll
       for (int u = 0; u < FLIGHT; ++u) {
-        const long long row = row0 + WAVES * u;
+        const long long row = row0 + WAVES * beside * u;
         if (row < end) {
           float y[V];
           if constexpr (!UPSTREAM) {
@@ -110,9 +114,12 @@ __global__ __launch_bounds__(kLayerRowsThreads, UPSTREAM ? 5 : 4) void LayerRows
   }
   if (p.bias_partials != nullptr) {
 #pragma unroll
-    for (int e = 0; e < V; ++e) { wave_sums[wave][lane * V + e] = sums[e]; }
+    for (int e = 0; e < V; ++e) {
+      for (int step = lanes; NARROW && step < 64; step *= 2) { sums[e] += __shfl_xor(sums[e], step, 64); }  // (rows side by side)
+      if (lane < lanes) { wave_sums[wave][lane * V + e] = sums[e]; }
+    }
     __syncthreads();
-    for (int i = threadIdx.x; i < 64 * V; i += kLayerRowsThreads) {
+    for (int i = threadIdx.x; i < lanes * V; i += kLayerRowsThreads) {
       const int feature = column_block * 64 * V + i;
       if (feature < p.m) {
         float sum = 0.0f;
@@ -163,13 +170,12 @@ __global__ __launch_bounds__(kLayerRowsThreads) void LayerAlignKernel(const Laye
 
 // out[group * out_stride + i] = the sum of the group's rows of `partials` (m values each): with offsets the tiles of `tile`
 // rows that the groups are cut into, numbered through from group 0 on; without, all `rows_of_sums` rows. Zero for a
-// group without a tile. grid: (ceil(m / 64), groups); the four wavefronts take every fourth row.
-template <typename T>
-__global__ __launch_bounds__(kLayerRowsThreads) void LayerColumnSumsKernel(const float* __restrict__ partials, const int rows_of_sums,
+// group without a tile. grid: (ceil(m / 64), groups); each of the WAVES wavefronts takes every WAVES-th row.
+template <typename T, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void LayerColumnSumsKernel(const float* __restrict__ partials, const int rows_of_sums,
                                                                            const int m, const long long* __restrict__ offsets,
                                                                            const int groups, const int rows, const int tile,
                                                                            T* __restrict__ out, const long long out_stride) {
-  constexpr int WAVES = kLayerRowsThreads / 64;
   __shared__ float wave_sums[WAVES][64];
   const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   for (int group = blockIdx.y; group < groups; group += gridDim.y) {

@@ -412,3 +412,36 @@ def test_two_graphs_of_one_stream(gpu):
         for t, want in zip((first, second, other), wanted):
             for name in OUTPUTS:
                 assert torch.equal(t[name], want[name]), name
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n", (1, 3, 8, 20, 129, 256, 300))
+def test_narrow_matrices_and_long_sums(gpu, dtype, n):
+    """Rows that take less than a wavefront side by side, with and without groups, whole and at odd places, against 64 bits. A
+    sum of p products of normal numbers in any order of fp32: p roundings of 2^-24 of a partial sum at most, which stays
+    below sum |.|, then its own rounding."""
+    half = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11, torch.float32: 2.0 ** -24}[dtype]
+    g = generator(50 + n)
+    m = 5003
+    y, z = (torch.randn(m, n + 2, generator=g, device="cuda:0").to(dtype) for _ in range(2))
+    c = torch.full((m, n + 2), 9.0, dtype=dtype, device="cuda:0")
+    bounds = [0, 0, 1, 700, 703, 703, 4990]
+    offsets = torch.tensor(bounds, device="cuda:0")
+    want = torch.where(z > 0, y, torch.zeros_like(y))  # relu: nothing is rounded
+    for groups in (None, offsets):
+        count = 1 if groups is None else len(bounds) - 1
+        ranges = [(0, m)] if groups is None else list(zip(bounds[:-1], bounds[1:]))
+        c.fill_(9.0)
+        sums = torch.full((count * n + 2,), 9.0, dtype=dtype, device="cuda:0")
+        api.activationGradient(None, m, n, y, z, c, n + 2, n + 2, n + 2, "relu", bias_gradient=sums, group_count=count, group_offsets=groups,
+                               y_offset=1, pre_offset=1, c_offset=1, bias_gradient_offset=1)
+        torch.cuda.synchronize()
+        assert torch.equal(c[:ranges[-1][1], 1:-1], want[:ranges[-1][1], 1:-1])
+        assert bool((c[:, 0] == 9.0).all()) and bool((c[:, -1] == 9.0).all()) and bool((c[ranges[-1][1]:] == 9.0).all())
+        assert float(sums[0]) == 9.0 and float(sums[-1]) == 9.0
+        for e, (begin, end) in enumerate(ranges):
+            part = want[begin:end, 1:-1].double()
+            exact, size = part.sum(0), part.abs().sum(0)
+            error = (sums[1 + e * n:1 + (e + 1) * n].double() - exact).abs()
+            bound = size * (end - begin) * 2.0 ** -24 * (1 + half) + exact.abs() * half + 2.0 ** -25
+            assert bool((error <= bound).all()), (e, float((error - bound).max()))
