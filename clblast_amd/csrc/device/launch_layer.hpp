@@ -100,6 +100,7 @@ int LaunchLayerProduct(const clbh_layer_desc& d, const LayerPlan& plan, const La
     case 4:
       if constexpr (!HALF) { return LaunchLayerConfig<LayerConfig<T, 4, 1, 1, 1, 4>>(d, plan, args, stream); }
       else { return hipErrorInvalidValue; }
+    case 5: return LaunchLayerConfig<LayerConfig<T, 2, 2, 1, 1, 4, HALF ? 5 : 3, 2>>(d, plan, args, stream);
     default: return LaunchLayerConfig<LayerConfig<T, 2, 2, 2, 2, 2, HALF ? 4 : 3>>(d, plan, args, stream);
   }
 }

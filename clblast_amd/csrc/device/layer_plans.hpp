@@ -18,7 +18,8 @@ namespace clbh {
 // (`alone`), its share when the compute unit is full of them (`full`), and the us that its start and epilogue keep
 // the compute unit from other work (`fixed`). Fitted on an MI355X to forced tiles at 256 .. 8192 x 4096 x 4096 and 8192^2 x 1024; a
 // tile that is alone on half of the compute units runs faster than one on all of them (the 16-bit products run against the
-// power limit), which the smallest tiles' k-walk, bound by latency, does not show.
+// power limit), which the smallest tiles' k-walk, bound by latency, does not show. The last one is the 64 x 64 tile whose depth two
+// sets of wavefronts share. On 40 random shapes the choice is 1.2 % behind the best of all forced ones, 17 % at worst.
 struct LayerTile {
   int variant, tile_m, tile_n, per_cu;
   double alone_16, full_16, fixed_16, alone_32, full_32, fixed_32;
@@ -27,6 +28,7 @@ constexpr LayerTile kLayerTiles[] = {
     {0, 128, 128, 2, 7.3, 9.3, 0.4, 61.6, 58.0, 2.0}, {1, 256, 256, 1, 17.0, 25.4, 4.5, 0.0, 0.0, 0.0},
     {2, 256, 128, 2, 15.0, 15.2, 1.5, 0.0, 0.0, 0.0}, {3, 64, 64, 4, 4.1, 3.7, 0.2, 16.8, 14.6, 0.3},
     {4, 128, 32, 4, 0.0, 0.0, 0.0, 18.5, 16.0, 0.3},
+    {5, 64, 64, 2, 3.6, 4.0, 0.3, 15.8, 14.6, 0.5},
 };
 constexpr int kLayerTileCount = sizeof(kLayerTiles) / sizeof(kLayerTiles[0]);
 

@@ -12,7 +12,7 @@
 // The offsets lie in device memory; they are clamped to the rows that exist, so no offset leads outside a matrix.
 //
 // Structure: a work-group owns a TILE_M x TILE_N tile, K is walked in slabs of 64 bytes per line (32 halfs, 16 floats) in a
-// ring of LDS buffers. Both types share the byte layout of a slab, the direct global -> LDS requests (16 bytes per lane, range-checked
+// ring of three to five LDS buffers. Both types share the byte layout of a slab, the direct global -> LDS requests (16 bytes per lane, range-checked
 // by the buffer resource), the one barrier per slab and the order of products: the wavefront's blocks form four quadrants
 // whose missing fragments are read under the products of the quadrant before. What differs is the instruction: 16 bits
 // v_mfma_f32_16x16x32_{f16,bf16}, a slab is one instruction deep, and x-contiguous operands are read with the transposing LDS
@@ -24,6 +24,18 @@
 // consecutive lanes along the features, so that bias, residual, Z and C all move in 16-byte pieces of whole lines, and a
 // lane keeps the same features for the whole tile (its bias values and its part of the bias gradient stay in registers).
 // Only the final value is rounded.
+//
+// What bounds it (bf16 and fp32, with the host's time per call where that is part of it): 8192 x 8192 x 4096 with bias, GELU and
+// stored Z 465 us, 1.18 PFLOP/s of the 1.29 that a large library product reaches here - the matrix pipe, and 4 us per
+// round of tiles for an epilogue under which nothing multiplies (a persistent form that loads the next tile under it held
+// both tiles' registers and was slower, 482 us). fp32 256 x 4096 x 4096 74 us, 116 of 154 TFLOP/s: the matrix pipe is busy for 74 to
+// 80 % of the cycles, the rest is a barrier per slab of 64 products of a block. Products of few rows: the weights' way from
+// memory, 64 experts of 128 rows 42 us for 201 MB. Small ones: the latency of a slab, about 0.15 us, times their number.
+//
+// Teams: few tiles of a long depth leave one work-group to a compute unit, whose four wavefronts wait for each slab. Two sets of
+// wavefronts with half the depth each, in one work-group, halve the number of slabs without a second kernel: 512 x 512 x 4096
+// in bf16 20.8 -> 18.9 us, 300 x 1000 x 512 in fp32 16.2 -> 14.1, 777 x 1001 x 1024 25.7 -> 22.3. With four tiles of 64 x 64
+// per compute unit the single set is ahead: 1024 x 4096 x 1024 in bf16 19.8 against 21.6.
 // =================================================================================================
 #ifndef CLBLAST_HIP_KERNELS_LAYER_GEMM_HPP_
 #define CLBLAST_HIP_KERNELS_LAYER_GEMM_HPP_
@@ -162,11 +174,13 @@ typedef float layer_float4_t __attribute__((ext_vector_type(4)));
 typedef float layer_float8_t __attribute__((ext_vector_type(8)));
 
 // WM x WN wavefronts, each owning (32 FM) x (32 FN) of the tile; BLOCK: extent of the matrix instruction's block.
-template <typename T_, int WM_, int WN_, int FM_, int FN_, int MIN_WAVES_, int STAGES_ = 3>
+// TEAMS = 2: two such sets of wavefronts with a ring each, of which the second takes the second half of the depth.
+template <typename T_, int WM_, int WN_, int FM_, int FN_, int MIN_WAVES_, int STAGES_ = 3, int TEAMS_ = 1>
 struct LayerConfig {
   using T = T_;
   static constexpr int WM = WM_, WN = WN_, FM = FM_, FN = FN_, MIN_WAVES = MIN_WAVES_;
-  static constexpr int WAVES = WM * WN, THREADS = 64 * WAVES;
+  static constexpr int TEAMS = TEAMS_;
+  static constexpr int WAVES = WM * WN, THREADS = 64 * WAVES * TEAMS;  // WAVES: of a team
   static constexpr int TILE_M = WM * FM * 32, TILE_N = WN * FN * 32;
   static constexpr int TILE_K = 64 / sizeof(T);
   static constexpr int VEC = 16 / sizeof(T);
@@ -182,9 +196,12 @@ struct LayerConfig {
   static constexpr int PITCH = WAVE_M + 4;  // floats of a row of the epilogue's staging tile
   static constexpr int HALF_N = WAVE_N / 2;  // rows that a wavefront stages at a time
   static constexpr int STAGE_BYTES = HALF_N * PITCH * 4;
-  static constexpr int EPILOGUE_BYTES = WAVES * STAGE_BYTES;
-  static constexpr int SUM_BYTES = WN * TILE_M * 4;  // the wavefronts' parts of the bias gradient
-  static constexpr int LDS_BYTES = (RING_BYTES > EPILOGUE_BYTES + SUM_BYTES) ? RING_BYTES : EPILOGUE_BYTES + SUM_BYTES;
+  static constexpr int EPILOGUE_BYTES = TEAMS * WAVES * STAGE_BYTES;
+  static constexpr int SUM_BYTES = TEAMS * WN * TILE_M * 4;  // the wavefronts' parts of the bias gradient
+  static constexpr int EXCHANGE_FLOATS = (TEAMS == 2) ? WAVE_M * HALF_N : 0;  // sums that a wavefront hands to the other team
+  static constexpr int TAIL_BYTES = EPILOGUE_BYTES + SUM_BYTES + TEAMS * WAVES * EXCHANGE_FLOATS * 4;
+  static constexpr int LDS_BYTES = (TEAMS * RING_BYTES > TAIL_BYTES) ? TEAMS * RING_BYTES : TAIL_BYTES;
+  static_assert(TEAMS == 1 || TEAMS == 2, "each team finishes one half of the rows");
   static_assert(BM % 2 == 0 && BN % 2 == 0 && BM >= BN, "the quadrants are halves of the blocks, walked along m");
 };
 
@@ -544,17 +561,18 @@ __global__ __launch_bounds__(Config::THREADS, Config::MIN_WAVES) void LayerGemmK
   using Acc = typename Math::Acc;
   constexpr int TILE_M = Config::TILE_M, TILE_N = Config::TILE_N, TILE_K = Config::TILE_K, BLOCK = Config::BLOCK;
   constexpr int BM = Config::BM, BN = Config::BN, HM = BM / 2, HN = BN / 2;
-  constexpr int WAVES = Config::WAVES, ROUNDS = Config::ROUNDS, STAGES = Config::STAGES, AHEAD = STAGES - 1;
+  constexpr int TEAMS = Config::TEAMS, WAVES = Config::WAVES, ROUNDS = Config::ROUNDS, STAGES = Config::STAGES, AHEAD = STAGES - 1;
   static_assert(AHEAD >= 2 && AHEAD <= 5 && AHEAD * ROUNDS < 64, "the waits below");
   using KernelTag = std::tuple<Config, std::integral_constant<int, (A_KC ? 2 : 0) | (B_KC ? 1 : 0)>>;
 
   extern __shared__ __align__(16) unsigned char lds_raw[];
-  char* a_ring = reinterpret_cast<char*>(lds_raw);
+  const int tid = threadIdx.x, lane = tid % 64;
+  const int any_wave = __builtin_amdgcn_readfirstlane(tid / 64);  // of both teams
+  const int wave = any_wave % WAVES, team = (TEAMS == 1) ? 0 : any_wave / WAVES;
+  char* a_ring = reinterpret_cast<char*>(lds_raw) + team * Config::RING_BYTES;
   char* b_ring = a_ring + STAGES * Config::A_BYTES;
   char* scratch_piece = b_ring + STAGES * Config::B_BYTES;
 
-  const int tid = threadIdx.x, lane = tid % 64;
-  const int wave = __builtin_amdgcn_readfirstlane(tid / 64);
   const int wave_m = wave % Config::WM, wave_n = wave / Config::WM;
 
   // ---- which tile, of which group
@@ -615,7 +633,15 @@ __global__ __launch_bounds__(Config::THREADS, Config::MIN_WAVES) void LayerGemmK
     for (int j = 0; j < BN; ++j) { acc[i][j] = Acc(0.0f); }
   }
 
-  const int slabs = (depth + TILE_K - 1) / TILE_K;
+  // Slabs of either team (both walk as many, they share the barriers; what lies behind the depth is zero)
+  const int slabs = ((depth + TILE_K - 1) / TILE_K + TEAMS - 1) / TEAMS;
+  const bool whole_slabs = depth % (TEAMS * TILE_K) == 0;
+  if (TEAMS == 2) {
+    const int before = team * slabs * TILE_K;
+    a += before * (A_KC ? 1 : p.a_ld);
+    b += before * (B_KC ? 1 : p.b_ld);
+    depth = max(0, min(slabs * TILE_K, depth - before));
+  }
   const int k_tail = depth % TILE_K;
   if (slabs > 0) {
     int a_offset[BM], b_offset[BN];
@@ -679,15 +705,18 @@ __global__ __launch_bounds__(Config::THREADS, Config::MIN_WAVES) void LayerGemmK
           LayerRequestPiece<true, KernelTag>(a_tile, a_tile, scratch_piece, lane * 16);
         }
       };
-      const auto zero_tail = [&](const int buffer) {
-        if (!RANGE || k_tail == 0 || !(A_KC || B_KC)) { return; }
+      // (one team: called for the last slab alone)
+      const auto zero_tail = [&](const int buffer, const int of_slab) {
+        if (!RANGE || !(A_KC || B_KC)) { return; }
+        const int k_valid = (TEAMS == 1) ? k_tail : max(0, min(TILE_K, depth - of_slab * TILE_K));
+        if (k_valid == ((TEAMS == 1) ? 0 : TILE_K)) { return; }
 #pragma unroll
         for (int round = 0; round < ROUNDS; ++round) {
           const int piece = wave + WAVES * round;
           if (piece < Config::PIECES_A) {
-            if (A_KC) { LayerZeroTail<T>(a_ring + buffer * Config::A_BYTES, piece, lane, k_tail); }
+            if (A_KC) { LayerZeroTail<T>(a_ring + buffer * Config::A_BYTES, piece, lane, k_valid); }
           } else if (piece < Config::PIECES_A + Config::PIECES_B) {
-            if (B_KC) { LayerZeroTail<T>(b_ring + buffer * Config::B_BYTES, piece - Config::PIECES_A, lane, k_tail); }
+            if (B_KC) { LayerZeroTail<T>(b_ring + buffer * Config::B_BYTES, piece - Config::PIECES_A, lane, k_valid); }
           }
         }
       };
@@ -707,7 +736,7 @@ __global__ __launch_bounds__(Config::THREADS, Config::MIN_WAVES) void LayerGemmK
       else if (first_slabs == 3) { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * ROUNDS) : "memory"); }
       else if (first_slabs == 4) { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(3 * ROUNDS) : "memory"); }
       else { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(4 * ROUNDS) : "memory"); }
-      if (slabs == 1) { zero_tail(0); }
+      if (TEAMS == 2 || slabs == 1) { zero_tail(0, 0); }
       __syncthreads();
       // 16 bits: halves of the fragments of one slab; fp32: all fragments of two slabs
       constexpr bool WIDE = sizeof(T) == 4;
@@ -716,7 +745,7 @@ __global__ __launch_bounds__(Config::THREADS, Config::MIN_WAVES) void LayerGemmK
       for (int q = 0; q < (WIDE ? BM : HM); ++q) { a_frag[0][q] = read_a(a_ring, q); }
 #pragma unroll
       for (int q = 0; q < (WIDE ? BN : HN); ++q) { b_frag[0][q] = read_b(b_ring, q); }
-      int cur = 0;
+      int cur = 0, slab = 0;
       // One slab; LATER: how many follow it, capped at AHEAD. Slab + AHEAD is requested under the first two quadrants, into the
       // buffer whose reads everybody had waited for at the previous barrier.
       constexpr int PER_SLOT = (ROUNDS + 2 * HM - 1) / (2 * HM);
@@ -733,7 +762,7 @@ __global__ __launch_bounds__(Config::THREADS, Config::MIN_WAVES) void LayerGemmK
           // slab + 1 must have landed for everybody; the requests for the slabs behind it may stay in flight
           constexpr int IN_FLIGHT = (LATER >= 2) ? (LATER - 1) * ROUNDS : 0;
           asm volatile("s_waitcnt vmcnt(%0)" ::"n"(IN_FLIGHT) : "memory");
-          if (LATER == 1) { zero_tail(nxt); }  // slab + 1 is the last one
+          if (LATER == 1 || (TEAMS == 2 && LATER > 1)) { zero_tail(nxt, slab + 1); }  // (LATER == 1: slab + 1 is the last one)
           asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
         };
         if constexpr (WIDE) {
@@ -802,7 +831,6 @@ __global__ __launch_bounds__(Config::THREADS, Config::MIN_WAVES) void LayerGemmK
           b_request += b_step;
         }
       };
-      int slab = 0;
       using Even = std::integral_constant<int, 0>;
       using Odd = std::integral_constant<int, WIDE ? 1 : 0>;
       using Steady = std::integral_constant<int, AHEAD>;
@@ -819,9 +847,11 @@ __global__ __launch_bounds__(Config::THREADS, Config::MIN_WAVES) void LayerGemmK
             if constexpr (LATER > 0) { self(self, std::integral_constant<int, LATER - 1>{}, parity_tag); }
           }
         };
-        for (; slab + AHEAD + 1 < slabs; slab += 2) {
+        while (slab + AHEAD + 1 < slabs) {
           slab_body(Steady{}, Even{});
+          ++slab;
           slab_body(Steady{}, Odd{});
+          ++slab;
         }
         if (slab + AHEAD < slabs) {
           slab_body(Steady{}, Even{});
@@ -843,8 +873,41 @@ __global__ __launch_bounds__(Config::THREADS, Config::MIN_WAVES) void LayerGemmK
         last_slabs(last_slabs, Last{});
       }
     };
-    if (m0 + TILE_M <= p.m && n0 + TILE_N <= rows && k_tail == 0) { walk(std::false_type{}); }
+    if (m0 + TILE_M <= p.m && n0 + TILE_N <= rows && whole_slabs) { walk(std::false_type{}); }
     else { walk(std::true_type{}); }
+  }
+
+  // ---- teams: each keeps one half of the rows and adds what the other one has of it
+  if constexpr (TEAMS == 2) {
+    float* exchange = reinterpret_cast<float*>(lds_raw + Config::EPILOGUE_BYTES + Config::SUM_BYTES);
+    float* given = exchange + (any_wave * Config::EXCHANGE_FLOATS + lane * 4);
+    const float* taken = exchange + ((wave + (1 - team) * WAVES) * Config::EXCHANGE_FLOATS + lane * 4);
+    constexpr int FOURS = sizeof(Acc) / 16;
+    __syncthreads();  // every wavefront is done with the slab buffers
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      if (half != team) {
+#pragma unroll
+        for (int i = 0; i < BM * HN * FOURS; ++i) {
+          layer_float4_t run;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) { run[e] = acc[i / FOURS % BM][half * HN + i / FOURS / BM][i % FOURS * 4 + e]; }
+          *reinterpret_cast<layer_float4_t*>(given + i * 256) = run;
+        }
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      if (half == team) {
+#pragma unroll
+        for (int i = 0; i < BM * HN * FOURS; ++i) {
+          const layer_float4_t run = *reinterpret_cast<const layer_float4_t*>(taken + i * 256);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) { acc[i / FOURS % BM][half * HN + i / FOURS / BM][i % FOURS * 4 + e] += run[e]; }
+        }
+      }
+    }
   }
 
   // ---- K ranges: the sums as they are
@@ -852,6 +915,7 @@ __global__ __launch_bounds__(Config::THREADS, Config::MIN_WAVES) void LayerGemmK
     float* partial = p.partials + static_cast<long long>(blockIdx.y) * p.n * p.m;
 #pragma unroll
     for (int j = 0; j < BN; ++j) {
+      if (TEAMS == 2 && j / HN != team) { continue; }
       const int row = n0 + (wave_n * BN + j) * BLOCK + lane % BLOCK;
 #pragma unroll
       for (int i = 0; i < BM; ++i) {
@@ -870,10 +934,10 @@ __global__ __launch_bounds__(Config::THREADS, Config::MIN_WAVES) void LayerGemmK
   }
 
   // ---- epilogue
-  __syncthreads();  // every wavefront is done with the slab buffers
+  if (TEAMS == 1) { __syncthreads(); }  // every wavefront is done with the slab buffers
   int late_lane = lane;  // (opaque, so that what the epilogue derives from it does not occupy registers during the walk)
   asm volatile("" : "+v"(late_lane));
-  float* stage = reinterpret_cast<float*>(lds_raw + wave * Config::STAGE_BYTES);
+  float* stage = reinterpret_cast<float*>(lds_raw + any_wave * Config::STAGE_BYTES);
   float* tile_sums = reinterpret_cast<float*>(lds_raw + Config::EPILOGUE_BYTES);
   const int wave_m0 = m0 + wave_m * Config::WAVE_M;
   const int inside = p.m - wave_m0;
@@ -902,6 +966,7 @@ __global__ __launch_bounds__(Config::THREADS, Config::MIN_WAVES) void LayerGemmK
     rows_of.Begin(bias, late_lane, inside);
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
+      if (TEAMS == 2 && half != team) { continue; }
 #pragma unroll
       for (int j = 0; j < HN; ++j) {
 #pragma unroll
@@ -924,14 +989,14 @@ __global__ __launch_bounds__(Config::THREADS, Config::MIN_WAVES) void LayerGemmK
       }
       wave_fence();
     }
-    if (p.bias_partials != nullptr) { rows_of.StoreSums(tile_sums + wave_n * TILE_M + wave_m * Config::WAVE_M, late_lane); }
+    if (p.bias_partials != nullptr) { rows_of.StoreSums(tile_sums + (team * Config::WN + wave_n) * TILE_M + wave_m * Config::WAVE_M, late_lane); }
   }
   if (p.bias_partials != nullptr) {
     __syncthreads();
     for (int i = tid; i < TILE_M && m0 + i < p.m; i += Config::THREADS) {
       float sum = tile_sums[i];
 #pragma unroll
-      for (int w = 1; w < Config::WN; ++w) { sum += tile_sums[w * TILE_M + i]; }
+      for (int w = 1; w < TEAMS * Config::WN; ++w) { sum += tile_sums[w * TILE_M + i]; }
       p.bias_partials[static_cast<long long>(sums_row) * p.m + m0 + i] = sum;
     }
   }

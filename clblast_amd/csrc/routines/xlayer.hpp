@@ -1,8 +1,8 @@
 // =================================================================================================
 // Xlayer<T>: host logic of the products of a network's layers - GemmEpilogue, GemmActivationGradient, ActivationGradient,
 // GemmGrouped and GemmGroupedGradient (include/clblast_hip.h). All matrices are row-major; the routines check the
-// arguments, read the row-major problem as the column-major one of the device layer (C^T = op(B)^T op(A)^T), copy an operand
-// that cannot be fetched in dwords into an aligned temporary and launch.
+// arguments, read the row-major problem as the column-major one of the device layer (C^T = op(B)^T op(A)^T) and launch;
+// the device layer copies an operand that cannot be fetched in dwords into the call's scratch memory.
 // T is float, half or bfloat16. The reference has no such routines.
 // =================================================================================================
 #ifndef CLBLAST_HIP_ROUTINES_XLAYER_HPP_

@@ -86,7 +86,7 @@ int main() {
     if (static_cast<double>(m) * n > 1e9) { continue; }
     clbh_layer_desc d{};
     d.type = type;
-    d.tile_variant = (form == 6) ? static_cast<int>(Random(6)) - 1 : -1;
+    d.tile_variant = (form == 6) ? static_cast<int>(Random(7)) - 1 : -1;
     d.split_k = (form == 6) ? static_cast<int>(Random(20)) : 0;
     d.m = m; d.n = n; d.k = k;
     d.a_kcontig = Random(2); d.b_kcontig = Random(2);

@@ -367,3 +367,47 @@ def test_offsets_that_lead_outside_are_clamped(gpu):
         api.gemmGroupedGradient(None, 4, m, k, n, a, c, result, offsets, k, n, n, k * n)
         torch.cuda.synchronize()
         assert bool((c[m:] == 5.0).all()) and bool((sums[4] == 0).all())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("split", (1, 3))
+def test_two_teams_along_the_depth(gpu, dtype, split):
+    """The tile whose depth two sets of wavefronts share: every parity of slabs, depths that leave the second set a part of a
+    slab or nothing, all transposes, sums in the bias gradient, groups"""
+    with Forced(dtype, 6, split):
+        for k in (1, 15, 16, 17, 31, 32, 33, 47, 48, 49, 63, 64, 65, 80, 95, 96, 97, 127, 128, 129, 160, 191, 192, 193, 320, 321, 1000):
+            for a_transp in (False, True):
+                for b_transp in (False, True):
+                    run_epilogue(dtype, 70, 66, k, a_transp, b_transp, "none", beta=1.0, seed=k)
+        run_epilogue(dtype, 256, 512, 128, False, True, "gelu", pre=True, beta=1.0)
+        run_epilogue(dtype, 301, 266, 330, False, True, "silu", pre=True, beta=1.0, in_place=True, seed=3)
+        run_gradient(dtype, 515, 300, 260, b_transp=True)
+        run_gradient(dtype, 256, 256, 256, a_transp=True, kind="silu", seed=2)
+        run_grouped(dtype, [300, 0, 17, 256, 1], 520, 200, 0, 3, True, "gelu", pre=True)
+        run_grouped(dtype, [31, 64, 300], 600, 96, 7, 0, False, "none", beta=1.0)
+        run_grouped_gradient(dtype, [300, 0, 17, 256, 1, 32, 33], 300, 520)
+        run_grouped_gradient(dtype, [300, 0, 17, 256, 1, 32, 33], 65, 66, 3, 5, beta=1.0)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_two_teams_read_nothing_beyond_the_depth(gpu, dtype):
+    """NaN behind every line of both operands, at depths that end inside a slab, at its end and before the second team's part"""
+    g = generator(60)
+    m, n = 70, 66
+    with Forced(dtype, 6, 1):
+        for k in (1, 7, 16, 33, 48, 64, 65, 97, 130):
+            for a_transp in (False, True):
+                for b_transp in (False, True):
+                    a_buffer, a = place(normal(g, *((k, m) if a_transp else (m, k))), dtype, (m if a_transp else k) + 66, 2)
+                    b_buffer, b = place(normal(g, *((n, k) if b_transp else (k, n))), dtype, (k if b_transp else n) + 66, 2)
+                    for buffer, view in ((a_buffer, a), (b_buffer, b)):
+                        values = view.clone()
+                        buffer.fill_(float("nan"))
+                        view.copy_(values)
+                    c = torch.zeros(m, n, dtype=dtype, device="cuda:0")
+                    api.gemmEpilogue(None, m, n, k, a_buffer, b_buffer, c, a.stride(0), b.stride(0), n, a_transp=a_transp, b_transp=b_transp,
+                                     a_offset=a.storage_offset(), b_offset=b.storage_offset())
+                    torch.cuda.synchronize()
+                    wide_a, wide_b = a.double(), b.double()
+                    want, bound, _, _ = ref.epilogue(wide_a.T if a_transp else wide_a, wide_b.T if b_transp else wide_b, dtype)
+                    ref.check(c, want, bound, "k = %d" % k)
