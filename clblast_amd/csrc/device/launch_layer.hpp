@@ -113,6 +113,7 @@ int LaunchLayerRowsOf(const clbh_layer_desc& d, const LayerPlan& plan, const Lay
   q.upstream_ld = d.upstream_ld;
   q.ranges = (d.upstream != nullptr) ? 1 : plan.splits;
   q.chunk = plan.rows_chunk;
+  q.row_blocks = static_cast<int>(plan.rows_chunks);
   q.lane_shift = plan.rows_lane_shift;
   const long long column_blocks = (static_cast<long long>(d.m) + 64 * V - 1) / (64 * V);
   if (column_blocks * plan.rows_chunks > INT_MAX) { return hipErrorInvalidConfiguration; }

@@ -51,6 +51,10 @@ __device__ __forceinline__ float NormalTail(const float z, float& bell) {
   }
 }
 
+// z, or zero where the factor that it meets is zero: an infinite z (a Z that overflowed 16 bits) has its limits, not infinity
+// times zero. A NaN comes in through that factor.
+__device__ __forceinline__ float Meeting(const float z, const float factor) { return (factor > 0.0f) ? z : 0.0f; }
+
 constexpr float kTanhSlope = 0.79788456f;  // sqrt(2 / pi)
 
 // act(z). `activation` is the same for the whole launch.
@@ -61,13 +65,17 @@ __device__ __forceinline__ float Activate(const int activation, const float z) {
     case kActivationGelu: {  // z Phi(z): z - z Phi(-z) on the positive side, z Phi(-|z|) on the other
       float bell;
       const float tail = NormalTail<FAST>(z, bell);
-      return __builtin_fmaf(-__builtin_fabsf(z), tail, (z < 0.0f) ? 0.0f : z);  // (a NaN stays one)
+      return __builtin_fmaf(-__builtin_fabsf(Meeting(z, tail)), tail, (z < 0.0f) ? 0.0f : z);  // (a NaN stays one)
     }
     case kActivationGeluTanh: {
       const float u = kTanhSlope * z * __builtin_fmaf(0.044715f * z, z, 1.0f);
-      return z * Reciprocal<FAST>(1.0f + Exponential<FAST>(-2.0f * u));
+      const float s = Reciprocal<FAST>(1.0f + Exponential<FAST>(-2.0f * u));
+      return Meeting(z, s) * s;
     }
-    case kActivationSilu: return z * Reciprocal<FAST>(1.0f + Exponential<FAST>(-z));
+    case kActivationSilu: {
+      const float s = Reciprocal<FAST>(1.0f + Exponential<FAST>(-z));
+      return Meeting(z, s) * s;
+    }
     default: return z;
   }
 }
@@ -80,7 +88,7 @@ __device__ __forceinline__ float ActivationSlope(const int activation, const flo
     case kActivationGelu: {
       float bell;
       const float tail = NormalTail<FAST>(z, bell);
-      return __builtin_fmaf(0.39894228f * z, bell, (z > 0.0f) ? 1.0f - tail : tail);  // 1 / sqrt(2 pi)
+      return __builtin_fmaf(0.39894228f * Meeting(z, bell), bell, (z > 0.0f) ? 1.0f - tail : tail);  // 1 / sqrt(2 pi)
     }
     case kActivationGeluTanh: {
       const float u = kTanhSlope * z * __builtin_fmaf(0.044715f * z, z, 1.0f);
@@ -94,7 +102,7 @@ __device__ __forceinline__ float ActivationSlope(const int activation, const flo
     case kActivationSilu: {
       const float s = Reciprocal<FAST>(1.0f + Exponential<FAST>(-z));
       const float r = Reciprocal<FAST>(1.0f + Exponential<FAST>(z));
-      return __builtin_fmaf(z * r, s, s);
+      return __builtin_fmaf(Meeting(z, s * r), s * r, s);
     }
     default: return 1.0f;
   }

@@ -28,9 +28,9 @@
 // What bounds it (bf16 and fp32, with the host's time per call where that is part of it): 8192 x 8192 x 4096 with bias, GELU and
 // stored Z 465 us, 1.18 PFLOP/s of the 1.29 that a large library product reaches here - the matrix pipe, and 4 us per
 // round of tiles for an epilogue under which nothing multiplies (a persistent form that loads the next tile under it held
-// both tiles' registers and was slower, 482 us). fp32 256 x 4096 x 4096 74 us, 116 of 154 TFLOP/s: the matrix pipe is busy for 74 to
+// both tiles' registers and was slower, 482 us). fp32 1024 x 1024 x 4096 74 us, 116 of 154 TFLOP/s: the matrix pipe is busy for 74 to
 // 80 % of the cycles, the rest is a barrier per slab of 64 products of a block. Products of few rows: the weights' way from
-// memory, 64 experts of 128 rows 42 us for 201 MB. Small ones: the latency of a slab, about 0.15 us, times their number.
+// memory, 128 rows over 64 experts of 2048 x 1024 in bf16 42 us for the 205 MB of the experts that have rows. Small ones: the latency of a slab, about 0.15 us, times their number.
 //
 // Teams: few tiles of a long depth leave one work-group to a compute unit, whose four wavefronts wait for each slab. Two sets of
 // wavefronts with half the depth each, in one work-group, halve the number of slabs without a second kernel: 512 x 512 x 4096
@@ -381,19 +381,27 @@ struct LayerPiece {
     for (int e = 0; e < V; ++e) { piece[e] = static_cast<T>(values[e]); }
     __builtin_nontemporal_store(piece, (GlobalPiece)(base + offset));
   }
-  // STREAM: what nobody reads a second time
-  template <bool STREAM = false>
   static __device__ __forceinline__ void Load(const T* from, const int inside, float (&values)[V]) {
     if (inside >= V) {
-      Piece piece;
-      if constexpr (STREAM) { piece = __builtin_nontemporal_load(reinterpret_cast<const Piece*>(from)); }
-      else { piece = *reinterpret_cast<const Piece*>(from); }
+      const Piece piece = *reinterpret_cast<const Piece*>(from);
 #pragma unroll
       for (int e = 0; e < V; ++e) { const T value = piece[e]; values[e] = static_cast<float>(value); }
     } else {
 #pragma unroll
       for (int e = 0; e < V; ++e) { values[e] = (e < inside) ? static_cast<float>(from[e]) : 0.0f; }
     }
+  }
+  // the same without the conversion, zeros behind `inside`. STREAM: what nobody reads a second time
+  template <bool STREAM>
+  static __device__ __forceinline__ Raw LoadRaw(const T* from, const int inside) {
+    if (inside >= V) {
+      if constexpr (STREAM) { return __builtin_bit_cast(Raw, __builtin_nontemporal_load(reinterpret_cast<const Piece*>(from))); }
+      else { return __builtin_bit_cast(Raw, *reinterpret_cast<const Piece*>(from)); }
+    }
+    Raw raw;
+#pragma unroll
+    for (int e = 0; e < V; ++e) { raw[e] = (e < inside) ? from[e] : T(0.0f); }
+    return raw;
   }
   static __device__ __forceinline__ void Store(T* to, const int inside, const float (&values)[V]) {
     if (inside >= V) {

@@ -4,7 +4,7 @@
 //     whose K range was split over several work-groups (added up here in the order of the ranges), or, for the gradient of
 //     an activation, a matrix of the caller's. One pass over memory; bound by it: GELU's gradient of 8192 x 8192 bf16 in
 //     74 us, 5.4 TB/s, the rate of a large copy (with one row in flight per wavefront 94, with four 231 - the compiler then spills -
-//     with the matrices kept in the caches 87; two rows at five wavefronts per SIMD are the most that the registers hold).
+//     with the matrices kept in the caches 87, with one register more than the 64 that eight wavefronts per SIMD leave 88).
 //   * LayerAlignKernel: copies of operands whose lines do not start at dwords, for the tiled kernel's loads.
 //   * LayerColumnSumsKernel: the second half of a bias gradient, which adds up the sums that the work-groups of either
 //     kernel left for their tiles of rows, in the order of the tiles: the result does not depend on timing.
@@ -23,7 +23,8 @@ struct LayerRowsArgs {
   const void* upstream;  // of the storage type, or nullptr: the fp32 sums at layer.partials
   long long upstream_ld;
   int ranges;            // K ranges at layer.partials
-  int chunk;             // rows per work-group
+  int chunk;             // rows per work-group: of a group consecutive ones; without groups `row_blocks` work-groups take turns
+  int row_blocks;
   int lane_shift;        // 2^lane_shift lanes per row, a wavefront takes 64 >> lane_shift rows side by side
   int column_blocks;     // work-groups side by side; the grid's only dimension counts them first
 };
@@ -33,7 +34,7 @@ struct LayerRowsArgs {
 // of the sums. NARROW: a row is the work of less than 64 lanes (65536 x 64 with all lanes on one row: 28 us, 9 like this;
 // 8192 x 8192 with row numbers in vector registers: 87 us, 74 with scalar ones).
 template <typename T, int V, bool UPSTREAM, bool NARROW>
-__global__ __launch_bounds__(kLayerRowsThreads, UPSTREAM ? 5 : 4) void LayerRowsKernel(const LayerRowsArgs q) {
+__global__ __launch_bounds__(kLayerRowsThreads, UPSTREAM ? 8 : 4) void LayerRowsKernel(const LayerRowsArgs q) {
   constexpr bool FAST = sizeof(T) == 2;
   constexpr int WAVES = kLayerRowsThreads / 64, FLIGHT = UPSTREAM ? 2 : 1;  // rows of a wavefront in flight together
   constexpr int RANGES = 8;                                                // K ranges in flight together
@@ -47,15 +48,17 @@ __global__ __launch_bounds__(kLayerRowsThreads, UPSTREAM ? 5 : 4) void LayerRows
   const int inside = p.m - col;  // features from this lane's first one on
 
   const int sums_row = blockIdx.x / q.column_blocks;
-  int first, end;
+  constexpr unsigned PASS = WAVES * FLIGHT;  // (times `beside`: the rows that a work-group takes together)
+  unsigned first, end, stride = PASS * beside;
   if (p.grouping == kLayerGroupedRows) {
     int group = 0, before = 0, begin = 0, last = 0;
     if (!FindGroupTile(p.offsets, p.groups, p.n, q.chunk, lane, [&](int) { return sums_row; }, group, before, begin, last)) { return; }
     first = begin + (sums_row - before) * q.chunk;
-    end = min(first + q.chunk, last);
+    end = min(first + q.chunk, static_cast<unsigned>(last));
   } else {
-    first = sums_row * q.chunk;
-    end = min(first + q.chunk, p.n);
+    first = sums_row * stride;
+    end = p.n;
+    stride *= q.row_blocks;  // (at most the rows and a chunk: what is added up stays below 2^32)
   }
 
   float bias[V], sums[V];
@@ -68,17 +71,21 @@ __global__ __launch_bounds__(kLayerRowsThreads, UPSTREAM ? 5 : 4) void LayerRows
   const long long other_ld = p.gradient ? p.pre_ld : p.residual_ld;
 
   if (inside > 0) {
-    for (int row0 = first + wave * beside + (NARROW ? lane >> lane_shift : 0); row0 < end; row0 += WAVES * FLIGHT * beside) {
-      float z[FLIGHT][V], old[FLIGHT][V];
+    for (unsigned row0 = first + wave * beside + (NARROW ? lane >> lane_shift : 0); row0 < end; row0 += stride) {
+      // (as they are in memory until their row's turn: half the registers of their values for 16 bits)
+      typename LayerPiece<T, V>::Raw upstream[FLIGHT], old[FLIGHT];
+      float z[V];
 #pragma unroll
       for (int u = 0; u < FLIGHT; ++u) {
-        const long long row = min(row0 + WAVES * beside * u, end - 1);  // (a row beyond the chunk: the last one again, not used)
+        const long long row = min(row0 + WAVES * beside * u, end - 1);  // (a row beyond the end: the last one again, not used)
 #pragma unroll
-        for (int e = 0; e < V; ++e) { z[u][e] = 0.0f; old[u][e] = 0.0f; }
-        if constexpr (UPSTREAM) { LayerPiece<T, V>::template Load<true>(static_cast<const T*>(q.upstream) + row * q.upstream_ld + col, inside, z[u]); }
-        if (other != nullptr) { LayerPiece<T, V>::template Load<UPSTREAM>(other + row * other_ld + col, inside, old[u]); }
+        for (int e = 0; e < V; ++e) { old[u][e] = T(0.0f); }
+        if constexpr (UPSTREAM) { upstream[u] = LayerPiece<T, V>::template LoadRaw<true>(static_cast<const T*>(q.upstream) + row * q.upstream_ld + col, inside); }
+        if (other != nullptr) { old[u] = LayerPiece<T, V>::template LoadRaw<UPSTREAM>(other + row * other_ld + col, inside); }
       }
       if constexpr (!UPSTREAM) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) { z[e] = 0.0f; }
         const float* from = p.partials + static_cast<long long>(row0) * p.m + col;
         const long long slab = static_cast<long long>(p.n) * p.m;
         for (int range = 0; range < q.ranges; range += RANGES) {
@@ -92,7 +99,7 @@ __global__ __launch_bounds__(kLayerRowsThreads, UPSTREAM ? 5 : 4) void LayerRows
 #pragma unroll
           for (int r = 0; r < RANGES; ++r) {
 #pragma unroll
-            for (int e = 0; e < V; ++e) { z[0][e] += more[r][e]; }
+            for (int e = 0; e < V; ++e) { z[e] += more[r][e]; }
           }
         }
       }
@@ -100,16 +107,18 @@ __global__ __launch_bounds__(kLayerRowsThreads, UPSTREAM ? 5 : 4) void LayerRows
       for (int u = 0; u < FLIGHT; ++u) {
         const long long row = row0 + WAVES * beside * u;
         if (row < end) {
-          float y[V];
+          float now[V], y[V];
+          LayerPiece<T, V>::Values(old[u], now);
+          if constexpr (UPSTREAM) { LayerPiece<T, V>::Values(upstream[u], z); }
           if constexpr (!UPSTREAM) {
 #pragma unroll
-            for (int e = 0; e < V; ++e) { z[u][e] = __builtin_fmaf(p.alpha, z[u][e], bias[e]); }
+            for (int e = 0; e < V; ++e) { z[e] = __builtin_fmaf(p.alpha, z[e], bias[e]); }
           }
-          LayerValues<FAST, true>(p, z[u], old[u], y);
+          LayerValues<FAST, true>(p, z, now, y);
 #pragma unroll
           for (int e = 0; e < V; ++e) { sums[e] += y[e]; }
           if (p.c != nullptr) { LayerPiece<T, V>::Store(static_cast<T*>(p.c) + row * p.c_ld + col, inside, y); }
-          if (!UPSTREAM && p.pre != nullptr && !p.gradient) { LayerPiece<T, V>::Store(static_cast<T*>(p.pre) + row * p.pre_ld + col, inside, z[u]); }
+          if (!UPSTREAM && p.pre != nullptr && !p.gradient) { LayerPiece<T, V>::Store(static_cast<T*>(p.pre) + row * p.pre_ld + col, inside, z); }
         }
       }
     }

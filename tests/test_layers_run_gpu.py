@@ -445,3 +445,24 @@ def test_narrow_matrices_and_long_sums(gpu, dtype, n):
             error = (sums[1 + e * n:1 + (e + 1) * n].double() - exact).abs()
             bound = size * (end - begin) * 2.0 ** -24 * (1 + half) + exact.abs() * half + 2.0 ** -25
             assert bool((error <= bound).all()), (e, float((error - bound).max()))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_activations_at_the_infinities(gpu, dtype):
+    """The limits of the functions and of their slopes; a NaN stays one"""
+    inf, nan = float("inf"), float("nan")
+    z = torch.tensor([[-inf, inf, nan, 0.0, -inf, inf, nan, 0.0]], device="cuda:0").to(dtype)
+    for kind, left, right in (("relu", 0.0, inf), ("gelu", 0.0, inf), ("gelu_tanh", 0.0, inf), ("silu", 0.0, inf), ("none", -inf, inf)):
+        for rows in (1, 300):  # an edge, and whole tiles
+            ones = torch.ones(rows, 1, device="cuda:0").to(dtype)
+            wide = z.repeat(1, 64).contiguous()
+            n = wide.shape[1]
+            c = torch.zeros(rows, n, dtype=dtype, device="cuda:0")
+            api.gemmEpilogue(None, rows, n, 1, ones, wide, c, 1, n, n, activation=kind)
+            torch.cuda.synchronize()
+            assert bool((c[:, 0::4] == left).all()) and bool((c[:, 1::4] == right).all()) and bool(c[:, 2::4].isnan().all()) and bool((c[:, 3::4] == 0).all()), kind
+        out = torch.zeros_like(z)
+        api.activationGradient(None, 1, 8, torch.ones_like(z), z, out, 8, 8, 8, activation=kind)
+        torch.cuda.synchronize()
+        assert float(out[0, 0]) == (1.0 if kind == "none" else 0.0) and float(out[0, 1]) == 1.0, (kind, out)
+        assert bool(out[0, 2].isnan()) or kind in ("relu", "none"), (kind, out)
