@@ -3,7 +3,7 @@
 //   * LayerRowsKernel: the epilogue of kernels/layer_gemm.hpp on sums that are already there - the fp32 sums of a product
 //     whose K range was split over several work-groups (added up here in the order of the ranges), or, for the gradient of
 //     an activation, a matrix of the caller's. One pass over memory; bound by it: GELU's gradient of 8192 x 8192 bf16 in
-//     74 us, 5.4 TB/s, the rate of a large copy (with one row in flight per wavefront 94, with four 231 - the compiler then spills -
+//     72 us, 5.6 TB/s, the rate of a large copy (with one row in flight per wavefront 94, with four 231 - the compiler then spills -
 //     with the matrices kept in the caches 87, with one register more than the 64 that eight wavefronts per SIMD leave 88).
 //   * LayerAlignKernel: copies of operands whose lines do not start at dwords, for the tiled kernel's loads.
 //   * LayerColumnSumsKernel: the second half of a bias gradient, which adds up the sums that the work-groups of either
@@ -23,15 +23,16 @@ struct LayerRowsArgs {
   const void* upstream;  // of the storage type, or nullptr: the fp32 sums at layer.partials
   long long upstream_ld;
   int ranges;            // K ranges at layer.partials
-  int chunk;             // rows per work-group: of a group consecutive ones; without groups `row_blocks` work-groups take turns
-  int row_blocks;
+  int chunk;             // rows per work-group
+  int row_blocks;        // work-groups along the rows where there are no groups
   int lane_shift;        // 2^lane_shift lanes per row, a wavefront takes 64 >> lane_shift rows side by side
   int column_blocks;     // work-groups side by side; the grid's only dimension counts them first
 };
 
-// Work-group: 64 pieces of V features (lanes; fewer of a narrow matrix, several rows side by side then) times `chunk` rows, which its
-// four wavefronts take in turn. bias_partials: one row of m sums for every chunk, the chunks numbered through the groups. UPSTREAM: the caller's matrix takes the place
-// of the sums. NARROW: a row is the work of less than 64 lanes (65536 x 64 with all lanes on one row: 28 us, 9 like this;
+// Work-group: 64 pieces of V features (lanes; fewer of a narrow matrix, several rows side by side then) times `chunk` rows; the work-groups
+// of a group (of the matrix) take its rows in turn, so that what is in flight at a time lies together (8192 x 8192 75 -> 72 us,
+// 8192 x 11008 115 -> 107; with its bias gradient 119 -> 111). bias_partials: one row of m sums for every work-group, numbered through
+// the groups. UPSTREAM: the caller's matrix takes the place of the sums. NARROW: a row is the work of less than 64 lanes (65536 x 64 with all lanes on one row: 28 us, 9 like this;
 // 8192 x 8192 with row numbers in vector registers: 87 us, 74 with scalar ones).
 template <typename T, int V, bool UPSTREAM, bool NARROW>
 __global__ __launch_bounds__(kLayerRowsThreads, UPSTREAM ? 8 : 4) void LayerRowsKernel(const LayerRowsArgs q) {
@@ -53,8 +54,9 @@ __global__ __launch_bounds__(kLayerRowsThreads, UPSTREAM ? 8 : 4) void LayerRows
   if (p.grouping == kLayerGroupedRows) {
     int group = 0, before = 0, begin = 0, last = 0;
     if (!FindGroupTile(p.offsets, p.groups, p.n, q.chunk, lane, [&](int) { return sums_row; }, group, before, begin, last)) { return; }
-    first = begin + (sums_row - before) * q.chunk;
-    end = min(first + q.chunk, static_cast<unsigned>(last));
+    first = begin + (sums_row - before) * stride;
+    end = last;
+    stride *= (last - begin + q.chunk - 1) / q.chunk;
   } else {
     first = sums_row * stride;
     end = p.n;
