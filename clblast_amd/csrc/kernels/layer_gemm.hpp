@@ -45,6 +45,7 @@
 #include "kernels/activations.hpp"
 #include "kernels/gemm_direct_f16.hpp"
 #include "kernels/gemm_mfma.hpp"
+#include "kernels/layer_requests.hpp"
 
 namespace clbh {
 
@@ -292,7 +293,7 @@ template <typename Config> struct LayerMathOf<Config, true> { using type = Layer
 // by (x >> 2) & 3; else lines k of W elements (16 bits: swizzled for the transposing read, fp32: in order).
 template <typename T, int W, bool KC>
 __device__ __forceinline__ int LayerPieceLaneBytes(const long long ld, const int piece, const int lane) {
-  constexpr int LINES = KC ? 16 : 1024 / (W * static_cast<int>(sizeof(T))), CHUNKS = 64 / LINES;
+  constexpr int LINES = LayerPieceLines(KC, W, sizeof(T)), CHUNKS = 64 / LINES;
   static_assert(LINES >= 1, "a piece holds whole lines");
   const int line = lane / CHUNKS, position = lane % CHUNKS;
   int chunk = position;
@@ -642,13 +643,16 @@ __global__ __launch_bounds__(Config::THREADS, Config::MIN_WAVES) void LayerGemmK
   }
 
   // Slabs of either team (both walk as many, they share the barriers; what lies behind the depth is zero)
-  const int slabs = ((depth + TILE_K - 1) / TILE_K + TEAMS - 1) / TEAMS;
+  const int slabs = LayerTeamSlabs(depth, TILE_K, TEAMS);
   const bool whole_slabs = depth % (TEAMS * TILE_K) == 0;
+  // behind the last element of the operand, taken before the teams part: the same for both
+  const char* a_end = reinterpret_cast<const char*>(a + LayerOperandElements(A_KC, p.m, depth, p.a_ld));
+  const char* b_end = reinterpret_cast<const char*>(b + LayerOperandElements(B_KC, rows, depth, p.b_ld));
   if (TEAMS == 2) {
-    const int before = team * slabs * TILE_K;
+    const int before = LayerTeamStart(depth, TILE_K, TEAMS, team);
     a += before * (A_KC ? 1 : p.a_ld);
     b += before * (B_KC ? 1 : p.b_ld);
-    depth = max(0, min(slabs * TILE_K, depth - before));
+    depth = LayerTeamDepth(depth, TILE_K, TEAMS, team);
   }
   const int k_tail = depth % TILE_K;
   if (slabs > 0) {
@@ -669,9 +673,6 @@ __global__ __launch_bounds__(Config::THREADS, Config::MIN_WAVES) void LayerGemmK
     constexpr long long SIZE = sizeof(T);
     const char* a_tile = reinterpret_cast<const char*>(a + (A_KC ? m0 * p.a_ld : static_cast<long long>(m0)));
     const char* b_tile = reinterpret_cast<const char*>(b + (B_KC ? n0 * p.b_ld : static_cast<long long>(n0)));
-    // behind the last element of the operand
-    const char* a_end = reinterpret_cast<const char*>(a + (A_KC ? (p.m - 1) * p.a_ld + depth : (depth - 1) * p.a_ld + p.m));
-    const char* b_end = reinterpret_cast<const char*>(b + (B_KC ? (rows - 1) * p.b_ld + depth : (depth - 1) * p.b_ld + rows));
 
     auto walk = [&](auto range_tag) {
       constexpr bool RANGE = decltype(range_tag)::value;
@@ -679,8 +680,7 @@ __global__ __launch_bounds__(Config::THREADS, Config::MIN_WAVES) void LayerGemmK
       const char* b_request = b_tile;
       const long long a_step = A_KC ? 64 : TILE_K * p.a_ld * SIZE;
       const long long b_step = B_KC ? 64 : TILE_K * p.b_ld * SIZE;
-      constexpr int A_LINES = A_KC ? 16 : 1024 / (TILE_M * static_cast<int>(SIZE));
-      constexpr int B_LINES = B_KC ? 16 : 1024 / (TILE_N * static_cast<int>(SIZE));
+      constexpr int A_LINES = LayerPieceLines(A_KC, TILE_M, SIZE), B_LINES = LayerPieceLines(B_KC, TILE_N, SIZE);
       const auto is_a = [&](const int round, const int piece) {
         return (Config::PIECES_A % WAVES == 0) ? (round < Config::PIECES_A / WAVES) : (piece < Config::PIECES_A);
       };
