@@ -312,6 +312,7 @@ typedef struct clbh_layer_desc_ {
 } clbh_layer_desc;
 // Scratch of one call: sums of K ranges, sums for the bias gradient, aligned copies of operands - 16-bit operands are fetched
 // in dwords, one whose lines start at odd elements (or whose leading dimension is CLBH_LAYER_MAX_LD or more) is copied first.
+// 0 for a descriptor that no plan can be made for (clbh_layer_launch refuses it).
 CLBH_API size_t clbh_layer_workspace_bytes(const clbh_layer_desc* desc);
 // Enqueues the kernels of one call. Returns 0 or the HIP error code.
 CLBH_API int clbh_layer_launch(const clbh_layer_desc* desc, hipStream_t stream);

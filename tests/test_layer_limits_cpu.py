@@ -1,9 +1,12 @@
-"""What the layer products may reach and what they refuse, without a GPU: the requests of every tile replayed on the host."""
+"""What the layer products may reach and what they refuse, without a GPU: the requests of every tile replayed on the host, and
+descriptors that the device layer's entry points have to turn down."""
 import os
 import shutil
 import subprocess
 
 import pytest
+
+from clblast_amd import _lib
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 CSRC = os.path.join(ROOT, "clblast_amd", "csrc")
@@ -25,3 +28,8 @@ def compiled(tmp_path, name, sources):
 def test_no_request_leaves_its_operand(tmp_path):
     """Depths of less than a slab among them: the second team of wavefronts then has nothing, and begins behind the operand"""
     compiled(tmp_path, "requests", [os.path.join(ROOT, "tests", "host", "layer_requests.cpp")])
+
+
+def test_descriptors_that_are_refused(tmp_path):
+    folder = os.path.dirname(_lib.LIB_PATH)
+    compiled(tmp_path, "descriptors", [os.path.join(ROOT, "tests", "host", "layer_descriptor.cpp"), "-L" + folder, "-lclblast_hip", "-Wl,-rpath," + folder])
