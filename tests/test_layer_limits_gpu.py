@@ -1,0 +1,46 @@
+"""The layer products at the edges of what they promise: how often a 16-bit result is not the nearest number."""
+import pytest
+import torch
+
+from clblast_amd import api
+from tests import layer_reference as ref
+
+pytestmark = pytest.mark.gpu
+
+
+def nearest(value, dtype):
+    """A 64-bit value rounded once. (The way over 32 bits rounds twice: it only matters within 2^-24 of a border, far less than the
+    errors that are counted here.)"""
+    return value.to(dtype)
+
+
+@pytest.mark.parametrize("kind,low", (("gelu", -4.0), ("silu", -4.0), ("gelu_tanh", -2.0)))
+def test_activations_are_nearly_always_rounded_to_nearest(gpu, kind, low):
+    """act(z) on the negative side, where its accuracy is that of its tail, for 16-bit results of half a million different z.
+    Off by e relative to its value, a result is rounded the wrong way where a border between two numbers lies within e of it: of
+    a value in [2^q, 2^(q + 1)) the borders are 2^(q - 10) apart in fp16 and 2^(q - 7) in bf16, so that is a share of at most
+    2 e 2^(q + 1) / 2^(q - 10) = 4096 e, or 512 e. e is 2^-20 at most: fit of Phi 2^-23.5, its evaluation and the hardware's
+    exponential and reciprocal a few times 2^-24, the rounded argument of the exponential, at most 11.6 (gelu at -4: z^2 log2(e) / 2),
+    3 (gelu_tanh at -2, of three roundings: 2u log2(e) is 5.4) or 5.8 (silu), times 2^-24 and less than that again for the rounded
+    log2(e): in all below 16 of 2^-24. Five standard deviations of a count are added."""
+    assert ref.FUNCTION[torch.float16] >= 2.0 ** -20
+    g = torch.Generator().manual_seed(8)
+    z = torch.arange(1, 1 << 14, dtype=torch.int32).to(torch.int16).view(torch.float16)
+    z = -z[(z > 0.04) & (z <= -low)].float()
+    n = z.numel() // 8 * 8
+    z = z[:n].to("cuda:0")
+    for dtype, share in ((torch.float16, 4096 * 2.0 ** -20), (torch.bfloat16, 512 * 2.0 ** -20)):
+        one = torch.ones(1, 1, dtype=dtype, device="cuda:0")
+        wrong = count = 0
+        rows = z.to(dtype).unique()
+        n = rows.numel()
+        for alpha in (0.5 + 0.5 * torch.rand(64 if dtype == torch.float16 else 512, generator=g)).tolist():
+            alpha = float(torch.tensor(alpha))
+            c = torch.zeros(1, n, dtype=dtype, device="cuda:0")
+            api.gemmEpilogue(None, 1, n, 1, one, rows, c, 1, n, n, alpha=alpha, activation=kind)
+            exact = ref.act((rows.float() * alpha).double(), kind)  # (alpha times a value is rounded once to 32 bits, here as there)
+            wrong += int((c[0] != nearest(exact, dtype)).sum())
+            count += n
+        most = share * count
+        print("%s %s: %d of %d not rounded to nearest, at most %.0f expected" % (kind, dtype, wrong, count, most))
+        assert wrong <= most + 5 * most ** 0.5 + 1, (kind, dtype, wrong, count, most)
