@@ -68,9 +68,11 @@ int LaunchLayerTile(const clbh_layer_desc& d, const LayerPlan& plan, const Layer
         hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds_bytes);
     if (attribute_status != hipSuccess) { return static_cast<int>(attribute_status); }
   }
-  kernel<<<dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(plan.splits)), dim3(Config::THREADS), lds_bytes, stream>>>(
-      args, static_cast<int>(plan.tiles_m), static_cast<int>(plan.tiles_n));
-  return static_cast<int>(hipGetLastError());
+  return LayerSlices(blocks, Config::THREADS, [&](const int first, const unsigned count) {
+    kernel<<<dim3(count, static_cast<unsigned>(plan.splits)), dim3(Config::THREADS), lds_bytes, stream>>>(
+        args, static_cast<int>(plan.tiles_m), static_cast<int>(plan.tiles_n), first);
+    return static_cast<int>(hipGetLastError());
+  });
 }
 
 template <typename Config>
@@ -116,7 +118,8 @@ int LaunchLayerRowsOf(const clbh_layer_desc& d, const LayerPlan& plan, const Lay
   q.row_blocks = static_cast<int>(plan.rows_chunks);
   q.lane_shift = plan.rows_lane_shift;
   const long long column_blocks = (static_cast<long long>(d.m) + 64 * V - 1) / (64 * V);
-  if (column_blocks * plan.rows_chunks > INT_MAX) { return hipErrorInvalidConfiguration; }
+  // (in one grid: a work-group has room for 32768 values at least, of which half exist, so that 2^32 threads would have 2^38)
+  if (column_blocks * plan.rows_chunks >= (1ll << 32) / kLayerRowsThreads) { return hipErrorInvalidConfiguration; }
   q.column_blocks = static_cast<int>(column_blocks);
   const auto kernel = (plan.rows_lane_shift < 6) ? LayerRowsKernel<T, V, UPSTREAM, true> : LayerRowsKernel<T, V, UPSTREAM, false>;
   kernel<<<dim3(static_cast<unsigned>(column_blocks * plan.rows_chunks)), dim3(kLayerRowsThreads), 0, stream>>>(q);
@@ -160,8 +163,10 @@ int AlignLayerOperands(const clbh_layer_desc& d, const LayerPlan& plan, LayerArg
   if (blocks[0] + blocks[1] == 0) { return 0; }
   if (blocks[0] + blocks[1] > INT_MAX) { return hipErrorInvalidConfiguration; }
   q.blocks_of_first = static_cast<int>(blocks[0]);
-  LayerAlignKernel<T><<<dim3(static_cast<unsigned>(blocks[0] + blocks[1])), dim3(kLayerRowsThreads), 0, stream>>>(q);
-  return static_cast<int>(hipGetLastError());
+  return LayerSlices(blocks[0] + blocks[1], kLayerRowsThreads, [&](const int first, const unsigned count) {
+    LayerAlignKernel<T><<<dim3(count), dim3(kLayerRowsThreads), 0, stream>>>(q, first);
+    return static_cast<int>(hipGetLastError());
+  });
 }
 
 template <typename T>
@@ -182,13 +187,15 @@ int LaunchLayerTyped(const clbh_layer_desc& d, const LayerPlan& plan, hipStream_
     const long long rows_of_sums = elementwise ? plan.rows_chunks : plan.tiles_n;
     const bool grouped = d.grouping == CLBH_GROUPS_BY_ROWS;
     const int groups = grouped ? d.groups : 1;
-    const dim3 grid(static_cast<unsigned>((static_cast<long long>(d.m) + 63) / 64), static_cast<unsigned>(groups < 65535 ? groups : 65535));
     const bool many = rows_of_sums >= 64ll * groups;  // sums per group
     const auto kernel = many ? LayerColumnSumsKernel<T, 16> : LayerColumnSumsKernel<T, 4>;
-    kernel<<<grid, dim3(many ? 1024 : 256), 0, stream>>>(
-        args.bias_partials, static_cast<int>(rows_of_sums), d.m, grouped ? d.offsets : nullptr, groups, d.n,
-        elementwise ? plan.rows_chunk : plan.tile.tile_n, static_cast<T*>(d.bias_gradient), static_cast<long long>(d.m));
-    return static_cast<int>(hipGetLastError());
+    const int threads = many ? 1024 : 256;
+    return LayerSlices((static_cast<long long>(d.m) + 63) / 64, threads, [&](const int first, const unsigned count) {
+      kernel<<<dim3(count, static_cast<unsigned>(groups < 65535 ? groups : 65535)), dim3(threads), 0, stream>>>(
+          args.bias_partials, static_cast<int>(rows_of_sums), d.m, grouped ? d.offsets : nullptr, groups, d.n,
+          elementwise ? plan.rows_chunk : plan.tile.tile_n, static_cast<T*>(d.bias_gradient), static_cast<long long>(d.m), first);
+      return static_cast<int>(hipGetLastError());
+    });
   }
   return 0;
 }

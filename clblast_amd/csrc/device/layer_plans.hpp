@@ -121,6 +121,19 @@ inline void ChooseLayerTile(const clbh_layer_desc& d, const int units, int& vari
   }
 }
 
+// A grid dimension takes less than 2^32 threads. A longer one - 2^30 rows of one feature, in tiles of 64 - goes out in slices of
+// 2^31 threads (a multiple of eight work-groups, so that these still meet the XCDs in turn): launch(first work-group, how many)
+// is called for each and returns 0, or an error that ends it.
+template <typename Launch>
+int LayerSlices(const long long blocks, const int threads, Launch&& launch) {
+  const long long most = (1ll << 31) / threads;
+  for (long long first = 0; first < blocks; first += most) {
+    const int status = launch(static_cast<int>(first), static_cast<unsigned>(std::min(most, blocks - first)));
+    if (status != 0) { return status; }
+  }
+  return 0;
+}
+
 inline LayerPlan PlanLayer(const clbh_layer_desc& d, const int units) {
   auto plan = LayerPlan{};
   plan.splits = 1;

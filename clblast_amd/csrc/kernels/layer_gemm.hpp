@@ -563,7 +563,7 @@ struct LayerRows {
 
 template <typename Config, bool A_KC, bool B_KC>
 __global__ __launch_bounds__(Config::THREADS, Config::MIN_WAVES) void LayerGemmKernel(const LayerArgs p, const int tiles_m,
-                                                                                     const int tiles_n) {
+                                                                                     const int tiles_n, const int first_block) {
   using T = typename Config::T;
   using Math = typename LayerMathOf<Config>::type;
   using Frag = typename Math::Frag;
@@ -583,6 +583,7 @@ __global__ __launch_bounds__(Config::THREADS, Config::MIN_WAVES) void LayerGemmK
   char* scratch_piece = b_ring + STAGES * Config::B_BYTES;
 
   const int wave_m = wave % Config::WM, wave_n = wave / Config::WM;
+  const unsigned block = first_block + blockIdx.x;  // (first_block: of this slice of the grid)
 
   // ---- which tile, of which group
   int tile_m, tile_n, group = 0;
@@ -592,8 +593,8 @@ __global__ __launch_bounds__(Config::THREADS, Config::MIN_WAVES) void LayerGemmK
     int before = 0, end = 0, index = 0;
     const bool found = FindGroupTile(p.offsets, p.groups, p.n, TILE_N, lane, [&](const int total) {
       const long long all = static_cast<long long>(total) * tiles_m;
-      if (static_cast<long long>(blockIdx.x) >= all || all > 0x7fffffff) { return -1; }
-      index = XcdContiguousIndex(blockIdx.x, total * tiles_m);
+      if (static_cast<long long>(block) >= all || all > 0x7fffffff) { return -1; }
+      index = XcdContiguousIndex(block, total * tiles_m);
       return index / tiles_m;
     }, group, before, first, end);
     if (!found) { return; }
@@ -609,15 +610,15 @@ __global__ __launch_bounds__(Config::THREADS, Config::MIN_WAVES) void LayerGemmK
     // The depths differ from group to group: every XCD (work-groups are dealt to the eight in turn) takes an eighth of every
     // group's tiles, a contiguous one, and the groups come in the order of their depths, the deepest first.
     const int share = (tiles_m * tiles_n + kNumXcd - 1) / kNumXcd;
-    const int local = static_cast<int>(blockIdx.x / kNumXcd) % share + static_cast<int>(blockIdx.x % kNumXcd) * share;
+    const int local = static_cast<int>(block / kNumXcd) % share + static_cast<int>(block % kNumXcd) * share;
     if (local >= tiles_m * tiles_n) { return; }
-    GroupOfRank(p.offsets, p.groups, p.k, blockIdx.x / kNumXcd / share, lane, group, first, depth);
+    GroupOfRank(p.offsets, p.groups, p.k, block / kNumXcd / share, lane, group, first, depth);
     const int walk = local / (8 * tiles_n), height = min(tiles_m - 8 * walk, 8);
     tile_m = 8 * walk + (local - walk * 8 * tiles_n) % height;
     tile_n = (local - walk * 8 * tiles_n) / height;
     sums_row = tile_n;
   } else {
-    TileOfBlock<(TILE_M >= 2 * TILE_N) ? 4 : 8>(blockIdx.x, gridDim.x, tiles_m, tiles_n, tile_m, tile_n);
+    TileOfBlock<(TILE_M >= 2 * TILE_N) ? 4 : 8>(block, tiles_m * tiles_n, tiles_m, tiles_n, tile_m, tile_n);
     sums_row = tile_n;
     if (p.split_chunk > 0) {
       first = blockIdx.y * p.split_chunk;

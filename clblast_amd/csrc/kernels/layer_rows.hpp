@@ -157,13 +157,14 @@ struct LayerAlignArgs {
   int blocks_of_first;  // the work-groups from this one on copy the second operand
 };
 template <typename T>
-__global__ __launch_bounds__(kLayerRowsThreads) void LayerAlignKernel(const LayerAlignArgs q) {
+__global__ __launch_bounds__(kLayerRowsThreads) void LayerAlignKernel(const LayerAlignArgs q, const int first_block) {
   constexpr int V = 16 / sizeof(T);
   typedef T Loose __attribute__((ext_vector_type(V), aligned(sizeof(T))));
   typedef T Tight __attribute__((ext_vector_type(V)));
-  const bool second = static_cast<int>(blockIdx.x) >= q.blocks_of_first;
+  const int grid_block = first_block + static_cast<int>(blockIdx.x);  // (first_block: of this slice of the grid)
+  const bool second = grid_block >= q.blocks_of_first;
   const LayerAlignOperand& o = q.operand[second ? 1 : 0];
-  const long long block = second ? blockIdx.x - q.blocks_of_first : blockIdx.x;
+  const long long block = second ? grid_block - q.blocks_of_first : grid_block;
   const long long line = ((block * kLayerRowsThreads + threadIdx.x) >> o.lane_shift);
   if (line >= static_cast<long long>(o.lines) * o.matrices) { return; }
   const int matrix = static_cast<int>(line / o.lines), in_matrix = static_cast<int>(line - static_cast<long long>(matrix) * o.lines);
@@ -183,12 +184,13 @@ __global__ __launch_bounds__(kLayerRowsThreads) void LayerAlignKernel(const Laye
 
 // out[group * out_stride + i] = the sum of the group's rows of `partials` (m values each): with offsets the tiles of `tile`
 // rows that the groups are cut into, numbered through from group 0 on; without, all `rows_of_sums` rows. Zero for a
-// group without a tile. grid: (ceil(m / 64), groups); each of the WAVES wavefronts takes every WAVES-th row.
+// group without a tile. grid: (ceil(m / 64), from `first_block` on, groups); each of the WAVES wavefronts takes every WAVES-th row.
 template <typename T, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void LayerColumnSumsKernel(const float* __restrict__ partials, const int rows_of_sums,
                                                                            const int m, const long long* __restrict__ offsets,
                                                                            const int groups, const int rows, const int tile,
-                                                                           T* __restrict__ out, const long long out_stride) {
+                                                                           T* __restrict__ out, const long long out_stride,
+                                                                           const int first_block) {
   __shared__ float wave_sums[WAVES][64];
   const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   for (int group = blockIdx.y; group < groups; group += gridDim.y) {
@@ -208,7 +210,7 @@ __global__ __launch_bounds__(64 * WAVES) void LayerColumnSumsKernel(const float*
       first = min(before, rows_of_sums);
       count = min((end - begin + tile - 1) / tile, rows_of_sums - first);
     }
-    const int feature = blockIdx.x * 64 + lane;
+    const int feature = (first_block + static_cast<int>(blockIdx.x)) * 64 + lane;
     float sum = 0.0f;
     if (feature < m) {
       const float* from = partials + static_cast<long long>(first) * m + feature;

@@ -1,5 +1,5 @@
 """What the layer products may reach and what they refuse, without a GPU: the requests of every tile replayed on the host, and
-descriptors that the device layer's entry points have to turn down."""
+descriptors that the device layer's entry points have to turn down, the plan at the largest sizes."""
 import os
 import shutil
 import subprocess
@@ -33,3 +33,7 @@ def test_no_request_leaves_its_operand(tmp_path):
 def test_descriptors_that_are_refused(tmp_path):
     folder = os.path.dirname(_lib.LIB_PATH)
     compiled(tmp_path, "descriptors", [os.path.join(ROOT, "tests", "host", "layer_descriptor.cpp"), "-L" + folder, "-lclblast_hip", "-Wl,-rpath," + folder])
+
+
+def test_plans_of_the_largest_sizes(tmp_path):
+    compiled(tmp_path, "limits", [os.path.join(ROOT, "tests", "host", "layer_limits.cpp")])

@@ -1,4 +1,5 @@
-"""The layer products at the edges of what they promise: how often a 16-bit result is not the nearest number."""
+"""The layer products at the edges of what they promise: how often a 16-bit result is not the nearest number, the largest
+numbers of rows and features."""
 import pytest
 import torch
 
@@ -44,3 +45,53 @@ def test_activations_are_nearly_always_rounded_to_nearest(gpu, kind, low):
         most = share * count
         print("%s %s: %d of %d not rounded to nearest, at most %.0f expected" % (kind, dtype, wrong, count, most))
         assert wrong <= most + 5 * most ** 0.5 + 1, (kind, dtype, wrong, count, most)
+
+
+def test_more_tiles_than_one_grid_holds(gpu):
+    """2^30 rows of one feature are 2^24 tiles of 64 rows, or 2^23 of 128, in 2^32 threads. A depth of one, so that every value is a
+    product alone: rounded once to fp16, by the product's fp32 sum exactly as by torch's."""
+    m = (1 << 30) + 77
+    g = torch.Generator(device="cuda:0").manual_seed(9)
+    a = torch.randn(m, 2, generator=g, device="cuda:0", dtype=torch.float16)  # (rows at dwords: nothing is copied)
+    b = torch.tensor([[1.25]], device="cuda:0", dtype=torch.float16)
+    for variant in (0, 4, 6, 1):
+        api.override_parameters(0, "Xlayer", 16, {"TILE_VARIANT": variant, "SPLIT_K": 0})
+        try:
+            c = torch.full((m + 3, 1), 7.0, device="cuda:0", dtype=torch.float16)
+            api.gemmEpilogue(None, m, 1, 1, a, b, c, 2, 1, 1)
+            torch.cuda.synchronize()
+        finally:
+            api.override_parameters(0, "Xlayer", 16, {"TILE_VARIANT": 0, "SPLIT_K": 0})
+        assert torch.equal(c[:m, 0], a[:, 0] * b[0, 0]), variant
+        assert bool((c[m:] == 7.0).all()), variant
+        del c
+
+
+def test_more_copied_lines_than_one_grid_holds(gpu):
+    """2^30 rows of 17 elements, every second of which starts between dwords: four threads copy one"""
+    m, k = (1 << 30) + 5, 17
+    a = torch.empty(m * k, device="cuda:0", dtype=torch.float16)  # 36.5 GB
+    part = torch.randn(1 << 20, k, generator=torch.Generator(device="cuda:0").manual_seed(10), device="cuda:0").round().half()
+    rows = a.view(m, k)
+    for at in range(0, m, 1 << 20):
+        rows[at:at + (1 << 20)] = part[:min(1 << 20, m - at)]
+    b = torch.ones(1, k, device="cuda:0", dtype=torch.float16)
+    c = torch.full((m + 3, 1), 7.0, device="cuda:0", dtype=torch.float16)
+    api.gemmEpilogue(None, m, 1, k, a, b, c, k, k, 1, b_transp=True)
+    torch.cuda.synchronize()
+    want = part.float().sum(1).half()  # (whole numbers: exact in any order)
+    for at in range(0, m, 1 << 20):
+        count = min(1 << 20, m - at)
+        assert torch.equal(c[at:at + count, 0], want[:count]), at
+    assert bool((c[m:] == 7.0).all())
+
+
+def test_more_columns_to_add_up_than_one_grid_holds(gpu):
+    """The sums of 2^30 features: 2^24 work-groups of 256 threads"""
+    n = (1 << 30) + 70
+    y = torch.randn(2, n, generator=torch.Generator(device="cuda:0").manual_seed(11), device="cuda:0", dtype=torch.float16)
+    sums = torch.full((n + 3,), 7.0, device="cuda:0", dtype=torch.float16)
+    api.activationGradient(None, 2, n, y, None, None, n, 0, 0, bias_gradient=sums)
+    torch.cuda.synchronize()
+    assert torch.equal(sums[:n], y[0] + y[1])  # (two values: one rounding)
+    assert bool((sums[n:] == 7.0).all())
