@@ -153,7 +153,7 @@ inline LayerPlan PlanLayer(const clbh_layer_desc& d, const int units) {
     if (d.split_k > 0) { wanted = d.split_k; }
     if (d.grouping == CLBH_GROUPS_NONE && wanted > 1) {
       const int chunk = static_cast<int>(((static_cast<long long>(d.k) + wanted - 1) / wanted + 63) / 64 * 64);
-      const int splits = (d.k + chunk - 1) / chunk;
+      const int splits = static_cast<int>((static_cast<long long>(d.k) + chunk - 1) / chunk);
       if (splits > 1 && splits <= 65535) {
         plan.splits = splits;
         plan.chunk = chunk;
@@ -165,7 +165,7 @@ inline LayerPlan PlanLayer(const clbh_layer_desc& d, const int units) {
   const long long per_block = 64ll * vector, column_blocks = (d.m + per_block - 1) / per_block;
   plan.rows_lane_shift = LayerRowsLaneShift(d.m, vector);
   plan.rows_chunk = LayerRowsChunk(d.n, column_blocks, plan.rows_lane_shift);
-  plan.rows_chunks = (d.grouping == CLBH_GROUPS_BY_ROWS) ? MostGroupTiles(d.n, d.groups, plan.rows_chunk) : (d.n + plan.rows_chunk - 1) / plan.rows_chunk;
+  plan.rows_chunks = (d.grouping == CLBH_GROUPS_BY_ROWS) ? MostGroupTiles(d.n, d.groups, plan.rows_chunk) : (static_cast<long long>(d.n) + plan.rows_chunk - 1) / plan.rows_chunk;
   if (d.bias_gradient != nullptr) {
     const long long rows_of_sums = (d.upstream != nullptr || plan.splits > 1) ? plan.rows_chunks : plan.tiles_n;
     plan.sums_offset = take(sizeof(float) * static_cast<size_t>(rows_of_sums) * static_cast<size_t>(d.m));

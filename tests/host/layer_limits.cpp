@@ -1,5 +1,6 @@
 // Host-only checks of the plan of the layer products (clblast_amd/csrc/device/layer_plans.hpp) at the largest sizes: no grid
-// dimension of 2^32 threads, every work-group of a grid in one slice.
+// dimension of 2^32 threads, every work-group of a grid in one slice, the work-groups' rows and the K ranges make up the
+// sizes up to the largest ones.
 // Compiled and run by tests/test_layer_limits_cpu.py.
 #include <cstdio>
 #include <initializer_list>
@@ -31,10 +32,49 @@ void CheckSlices() {
     if (clbh::LayerSlices(2 * most, threads, [&](int, unsigned) { ++calls; return 7; }) != 7 || calls != 1) { Violation("an error ends the launches", calls); }
   }
 }
+
+void CheckLargest() {
+  char* const place = reinterpret_cast<char*>(4096);
+  constexpr int kMost = static_cast<int>(CLBH_LAYER_MAX_SIZE);
+  for (const int type : {CLBH_TYPE_FP16, CLBH_TYPE_FP32, CLBH_TYPE_BF16})
+  for (const int large : {kMost, kMost - 1, kMost - 4097, kMost - 9000, 1 << 30, (1 << 30) + 1})
+  for (const int small : {1, 2, 8, 9, 17, 64}) {
+    ++cases;
+    clbh_layer_desc d{};
+    d.type = type;
+    d.tile_variant = -1;
+    d.m = small; d.n = large; d.k = 1;
+    d.gradient = 1;
+    d.activation = 161;
+    d.upstream = d.c = d.bias_gradient = place;
+    d.upstream_ld = d.c_ld = small;
+    const auto rows = clbh::PlanLayer(d, 256);  // elementwise, many rows
+    if (rows.rows_chunk < 1 || rows.rows_chunks * rows.rows_chunk < large || (rows.rows_chunks - 1) * rows.rows_chunk >= large) { Violation("chunks of rows", rows.rows_chunks); }
+    if (rows.workspace_bytes < sizeof(float) * rows.rows_chunks * small || rows.workspace_bytes > sizeof(float) * rows.rows_chunks * small + 256) { Violation("workspace of the sums", static_cast<long long>(rows.workspace_bytes)); }
+    d.upstream = nullptr;
+    d.gradient = 0;
+    d.bias_gradient = nullptr;
+    d.a = d.b = place;
+    for (const bool deep : {false, true}) {  // products of many rows, and of a long depth
+      d.n = deep ? small : large;
+      d.k = deep ? large : small;
+      d.a_kcontig = d.b_kcontig = 1;
+      d.a_ld = d.b_ld = d.k;
+      for (const int split : {0, 2, 3, 7, 32}) {
+        d.split_k = split;
+        const auto plan = clbh::PlanLayer(d, 256);
+        if (plan.tiles_n * plan.tile.tile_n < d.n || (plan.tiles_n - 1) * plan.tile.tile_n >= d.n) { Violation("tiles along the rows", plan.tiles_n); }
+        if (plan.splits < 1 || (split > 1 && deep && plan.splits != split)) { Violation("K ranges", plan.splits); }
+        if (plan.splits > 1 && (static_cast<long long>(plan.chunk) * plan.splits < d.k || static_cast<long long>(plan.chunk) * (plan.splits - 1) >= d.k)) { Violation("length of the K ranges", plan.chunk); }
+      }
+    }
+  }
+}
 }  // namespace
 
 int main() {
   CheckSlices();
+  CheckLargest();
   std::printf("cases %lld violations %lld\n", cases, violations);
   return violations == 0 ? 0 : 1;
 }

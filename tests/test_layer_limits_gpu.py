@@ -95,3 +95,39 @@ def test_more_columns_to_add_up_than_one_grid_holds(gpu):
     torch.cuda.synchronize()
     assert torch.equal(sums[:n], y[0] + y[1])  # (two values: one rounding)
     assert bool((sums[n:] == 7.0).all())
+
+
+def test_the_most_rows_of_a_narrow_matrix(gpu):
+    m = (1 << 31) - 1024
+    y = torch.randn(m, generator=torch.Generator(device="cuda:0").manual_seed(12), device="cuda:0", dtype=torch.float16).sign_()
+    y[5], y[-1] = 0.0, 0.0
+    c = torch.full((m + 3,), 7.0, device="cuda:0", dtype=torch.float16)
+    sums = torch.full((3,), 7.0, device="cuda:0", dtype=torch.float16)
+    api.activationGradient(None, m, 1, y, y, c, 1, 1, 1, "relu", bias_gradient=sums)
+    torch.cuda.synchronize()
+    assert torch.equal(c[:m], y.clamp(min=0)) and bool((c[m:] == 7.0).all())
+    # (about 2^30 ones: more than fp16 holds)
+    assert float(sums[0]) == float("inf") and bool((sums[1:] == 7.0).all())
+
+
+def test_the_longest_depth(gpu):
+    """One row by one column of 2^31 - 1024 elements in K ranges; ones at both ends and at the borders of the ranges, so that the
+    sum counts what was multiplied (and stays below 2^11, a whole number that fp16 holds)"""
+    k = (1 << 31) - 1024
+    a, b = (torch.zeros(k, device="cuda:0", dtype=torch.float16) for _ in range(2))
+    places = {0, 1, 63, 64, k - 1, k - 2, k - 1024, 1 << 30, (1 << 30) - 1}
+    for ranges in (31, 32):
+        length = ((k + ranges - 1) // ranges + 63) // 64 * 64
+        for r in range(1, ranges):
+            places.update(range(r * length - 3, r * length + 3))
+    index = torch.tensor(sorted(places), device="cuda:0")
+    a[index], b[index] = 1.0, 1.0
+    for split, turned in ((0, False), (31, True), (32, False)):
+        api.override_parameters(0, "Xlayer", 16, {"TILE_VARIANT": 0, "SPLIT_K": split})
+        try:
+            c = torch.zeros(1, device="cuda:0", dtype=torch.float16)
+            api.gemmEpilogue(None, 1, 1, k, a, b, c, 1 if turned else k, k if turned else 1, 1, a_transp=turned, b_transp=turned)
+            torch.cuda.synchronize()
+        finally:
+            api.override_parameters(0, "Xlayer", 16, {"TILE_VARIANT": 0, "SPLIT_K": 0})
+        assert float(c) == len(places), (split, float(c), len(places))
