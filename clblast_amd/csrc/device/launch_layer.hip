@@ -17,6 +17,7 @@ bool ValidSizes(const clbh_layer_desc& d) {
   if (d.type != CLBH_TYPE_FP16 && d.type != CLBH_TYPE_BF16 && d.type != CLBH_TYPE_FP32) { return false; }
   if (d.m <= 0 || d.n <= 0 || (d.k <= 0 && d.upstream == nullptr)) { return false; }
   if (d.m > CLBH_LAYER_MAX_SIZE || d.n > CLBH_LAYER_MAX_SIZE || d.k > CLBH_LAYER_MAX_SIZE) { return false; }
+  if (!clbh::LayerOperandsReachable(d)) { return false; }
   if (d.grouping == CLBH_GROUPS_NONE) { return true; }
   if (d.grouping != CLBH_GROUPS_BY_ROWS && d.grouping != CLBH_GROUPS_BY_DEPTH) { return false; }
   if (d.groups <= 0 || d.groups > CLBH_LAYER_MAX_GROUPS) { return false; }

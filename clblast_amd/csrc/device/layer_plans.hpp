@@ -52,6 +52,26 @@ inline bool LayerOperandFits(const void* pointer, const long long ld, const long
   return type == CLBH_TYPE_FP32 || (reinterpret_cast<unsigned long long>(pointer) % 4 == 0 && ld % 2 == 0 && stride % 2 == 0);
 }
 
+// The leading dimension of an operand's copy
+inline long long LayerCopyLd(const long long length) { return (length + 7) / 8 * 8; }
+
+// A slab's pieces reach their lines - sixteen rows or features of a k-contiguous operand, up to eight depths of another - by
+// unsigned 32-bit byte offsets. Where these do not suffice for a copy without padding either, there is no launch for the operand. Rows
+// and features that do not exist may wrap: what they fetch lies inside the operand and is not stored. Depths may not, they have
+// to read as zero.
+inline bool LayerLinesReachable(const bool k_contiguous, const long long lines, const long long ld, const int type) {
+  const long long last = (k_contiguous ? std::min(lines, 16ll) : 8) - 1, size = (type == CLBH_TYPE_FP32) ? 4 : 2;
+  return last * ld * size + 512 <= 1ll << 32;
+}
+inline bool LayerOperandsReachable(const clbh_layer_desc& d) {
+  if (d.upstream != nullptr) { return true; }
+  const auto reachable = [&](const int k_contiguous, const long long across) {
+    const long long length = k_contiguous ? d.k : across, lines = k_contiguous ? across : d.k;
+    return LayerLinesReachable(k_contiguous != 0, lines, LayerCopyLd(length), d.type);
+  };
+  return reachable(d.a_kcontig, d.m) && reachable(d.b_kcontig, d.n);
+}
+
 // Most tiles of `tile` rows that `groups` ranges within `rows` rows can be cut into: every group can add one that is not full
 inline long long MostGroupTiles(const long long rows, const long long groups, const long long tile) {
   return std::min(rows, (rows + groups * (tile - 1)) / tile);
@@ -174,11 +194,11 @@ inline LayerPlan PlanLayer(const clbh_layer_desc& d, const int units) {
     const size_t size = (d.type == CLBH_TYPE_FP32) ? 4 : 2;
     const bool by_rows = d.grouping == CLBH_GROUPS_BY_ROWS;
     if (!LayerOperandFits(d.a, d.a_ld, by_rows ? d.a_stride : 0, d.type)) {
-      plan.a_copy_ld = ((d.a_kcontig ? d.k : d.m) + 7ll) / 8 * 8;
+      plan.a_copy_ld = LayerCopyLd(d.a_kcontig ? d.k : d.m);
       plan.a_copy_offset = take(size * static_cast<size_t>(plan.a_copy_ld) * static_cast<size_t>(d.a_kcontig ? d.m : d.k) * static_cast<size_t>((by_rows && d.a_stride != 0) ? d.groups : 1));
     }
     if (!LayerOperandFits(d.b, d.b_ld, 0, d.type)) {
-      plan.b_copy_ld = ((d.b_kcontig ? d.k : d.n) + 7ll) / 8 * 8;
+      plan.b_copy_ld = LayerCopyLd(d.b_kcontig ? d.k : d.n);
       plan.b_copy_offset = take(size * static_cast<size_t>(plan.b_copy_ld) * static_cast<size_t>(d.b_kcontig ? d.n : d.k));
     }
   }

@@ -299,7 +299,7 @@ __device__ __forceinline__ int LayerPieceLaneBytes(const long long ld, const int
   int chunk = position;
   if constexpr (KC) { chunk = position ^ ((line >> 2) & 3); }
   else if constexpr (sizeof(T) == 2) { chunk = position ^ HSwizzle<W>(LINES * piece + line); }
-  return static_cast<int>(line * ld * static_cast<long long>(sizeof(T))) + 16 * chunk;
+  return static_cast<int>(static_cast<unsigned>(line * ld * static_cast<long long>(sizeof(T)) + 16 * chunk));  // (the load takes it as unsigned)
 }
 
 template <bool RANGE, typename Tag>

@@ -5,6 +5,8 @@
 
 #include <memory>
 
+#include "device/layer_plans.hpp"
+
 namespace clblast {
 // =================================================================================================
 namespace {
@@ -265,6 +267,7 @@ void Xlayer<T>::DoGemmGroupedGradient(const size_t m, const size_t n, const size
 
 template <typename T>
 void Xlayer<T>::Launch(clbh_layer_desc& desc) {
+  if (!clbh::LayerOperandsReachable(desc)) { throw BLASError(StatusCode::kInvalidDimension, "rows of an operand are too long"); }
   ApplyLayerOverrides(sizeof(T) == 4 ? Precision::kSingle : Precision::kHalf, desc.tile_variant, desc.split_k);
   std::unique_ptr<StreamScratch> scratch;
   desc.workspace_bytes = clbh_layer_workspace_bytes(&desc);

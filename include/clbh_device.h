@@ -277,7 +277,7 @@ CLBH_API int clbh_conv_slab(int precision, const clbh_im2col_shape* shape, int k
 #define CLBH_GROUPS_NONE 0
 #define CLBH_GROUPS_BY_ROWS 1
 #define CLBH_GROUPS_BY_DEPTH 2
-#define CLBH_LAYER_MAX_LD (1ll << 23)        // operands: 16 lines of a slab stay at 32-bit byte offsets
+#define CLBH_LAYER_MAX_LD (1ll << 23)        // operands: lines further apart are copied first (LayerLinesReachable: which copies will do)
 #define CLBH_LAYER_MAX_GROUPED (1ll << 26)   // rows (depths) of a grouped call
 #define CLBH_LAYER_MAX_GROUPS (1ll << 16)    // every work-group looks through all of them
 #define CLBH_LAYER_MAX_SIZE ((1ll << 31) - 1024)  // m, n, k: a tile that begins inside ends below 2^31
@@ -310,6 +310,8 @@ typedef struct clbh_layer_desc_ {
   void* workspace;   // clbh_layer_workspace_bytes(desc) bytes, 256-byte aligned
   size_t workspace_bytes;
 } clbh_layer_desc;
+// A slab's lines - 16 rows or features that are k-contiguous (as many as there are), 8 depths otherwise - lie within 2^32 bytes once
+// they are copied without padding: an operand whose lines are longer has no launch.
 // Scratch of one call: sums of K ranges, sums for the bias gradient, aligned copies of operands - 16-bit operands are fetched
 // in dwords, one whose lines start at odd elements (or whose leading dimension is CLBH_LAYER_MAX_LD or more) is copied first.
 // 0 for a descriptor that no plan can be made for (clbh_layer_launch refuses it).

@@ -71,6 +71,21 @@ int main() {
     (grouping == CLBH_GROUPS_BY_ROWS ? d.n : d.k) = 1 << 26;
     Refused("rows of a grouped call", d);
   }
+  for (const int type : {CLBH_TYPE_FP16, CLBH_TYPE_FP32}) {  // lines that no 32-bit offset reaches
+    auto d = Good(CLBH_GROUPS_NONE);
+    d.type = type;
+    d.k = (type == CLBH_TYPE_FP32 ? 1 << 26 : 1 << 27) + (1 << 24);
+    d.m = 16;
+    d.a_kcontig = 1;
+    d.a_ld = d.k;
+    Refused("k-contiguous lines", d);
+    d = Good(CLBH_GROUPS_NONE);
+    d.type = type;
+    d.n = type == CLBH_TYPE_FP32 ? 160000000 : 320000000;
+    d.k = 1;
+    d.b_ld = d.n;
+    Refused("lines of rows", d);
+  }
   for (const int grouping : {-1, 3, 2147483647}) { Refused("grouping", Good(grouping)); }
   std::printf("cases %d violations %d\n", cases, violations);
   return violations == 0 ? 0 : 1;

@@ -1,6 +1,6 @@
 // Host-only checks of the plan of the layer products (clblast_amd/csrc/device/layer_plans.hpp) at the largest sizes: no grid
 // dimension of 2^32 threads, every work-group of a grid in one slice, the work-groups' rows and the K ranges make up the
-// sizes up to the largest ones.
+// sizes up to the largest ones, lines that are too far apart for 32-bit offsets are told from those that are not.
 // Compiled and run by tests/test_layer_limits_cpu.py.
 #include <cstdio>
 #include <initializer_list>
@@ -70,9 +70,34 @@ void CheckLargest() {
     }
   }
 }
+
+// The offsets of a piece's lines as the loads take them, unsigned and in 32 bits: of every line that counts it is the true one
+void CheckReach() {
+  for (const int type : {CLBH_TYPE_FP16, CLBH_TYPE_FP32, CLBH_TYPE_BF16})
+  for (const bool k_contiguous : {false, true})
+  for (const long long lines : {1ll, 2ll, 3ll, 8ll, 9ll, 16ll, 17ll, 1000ll}) {
+    const long long size = type == CLBH_TYPE_FP32 ? 4 : 2;
+    const auto wraps = [&](const long long ld) {
+      for (long long line = 0; line < (k_contiguous ? 16 : 8); ++line) {
+        if (k_contiguous && line >= lines) { break; }  // (what a row that does not exist fetches is not stored)
+        const long long last = line * ld * size + 511;
+        if (static_cast<long long>(static_cast<unsigned>(last)) != last) { return true; }
+      }
+      return false;
+    };
+    for (long long ld = 8; ld < 1ll << 33; ld = ld * 5 / 4 / 8 * 8 + 8) {
+      ++cases;
+      if (clbh::LayerLinesReachable(k_contiguous, lines, ld, type) == wraps(ld)) { Violation("lines within reach", ld); }
+    }
+  }
+  for (const long long length : {1ll, 8ll, 9ll, 16ll, 2147482624ll}) {
+    if (clbh::LayerCopyLd(length) < length || clbh::LayerCopyLd(length) % 8 != 0) { Violation("leading dimension of a copy", length); }
+  }
+}
 }  // namespace
 
 int main() {
+  CheckReach();
   CheckSlices();
   CheckLargest();
   std::printf("cases %lld violations %lld\n", cases, violations);

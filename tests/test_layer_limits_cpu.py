@@ -1,5 +1,6 @@
 """What the layer products may reach and what they refuse, without a GPU: the requests of every tile replayed on the host, and
-descriptors that the device layer's entry points have to turn down, the plan at the largest sizes."""
+descriptors that the device layer's entry points have to turn down, the plan at the largest sizes, the argument checks with
+buffers of any size."""
 import os
 import shutil
 import subprocess
@@ -37,3 +38,8 @@ def test_descriptors_that_are_refused(tmp_path):
 
 def test_plans_of_the_largest_sizes(tmp_path):
     compiled(tmp_path, "limits", [os.path.join(ROOT, "tests", "host", "layer_limits.cpp")])
+
+
+def test_calls_that_are_told_apart(tmp_path):
+    compiled(tmp_path, "calls", [os.path.join(ROOT, "tests", "host", "layer_calls.cpp")] +
+             [os.path.join(CSRC, "routines", name) for name in ("xlayer.cpp", "xgemm.cpp", "routine_common.cpp", "tile_table.cpp")])

@@ -131,3 +131,37 @@ def test_the_longest_depth(gpu):
         finally:
             api.override_parameters(0, "Xlayer", 16, {"TILE_VARIANT": 0, "SPLIT_K": 0})
         assert float(c) == len(places), (split, float(c), len(places))
+
+
+def test_lines_up_to_the_reach_of_32_bits(gpu):
+    """17 rows of the longest that 16 rows may have (the sixteenth 4.3e9 bytes behind the first); ones where both operands have
+    them count what was multiplied. A piece more is refused. Then features as many as eight depths reach."""
+    m, k = 17, 143165552
+    a, b = torch.zeros(m, k, device="cuda:0", dtype=torch.float16), torch.zeros(2, k, device="cuda:0", dtype=torch.float16)
+    places = torch.tensor([0, 1, 31, 32, 12345678, k // 2, k - 33, k - 2, k - 1], device="cuda:0")
+    b[0, places] = 1.0
+    b[1, places[:4]] = 2.0
+    for row in range(m):
+        a[row, places[:1 + row % 9]] = 1.0 + row
+    c = torch.zeros(m, 2, device="cuda:0", dtype=torch.float16)
+    api.gemmEpilogue(None, m, 2, k, a, b, c, k, k, 2, b_transp=True)
+    torch.cuda.synchronize()
+    want = [[(1 + row) * (1 + row % 9), (1 + row) * 2 * min(4, 1 + row % 9)] for row in range(m)]
+    assert c.tolist() == want
+    long = torch.zeros(m * (k + 16), device="cuda:0", dtype=torch.float16)
+    with pytest.raises(api.CLBlastError) as error:
+        api.gemmEpilogue(None, m, 1, k + 16, long, long, c, k + 16, k + 16, 1, b_transp=True)
+    assert error.value.status == -1017
+    del a, b, long
+    n, k = 306783328, 9
+    g = torch.Generator(device="cuda:0").manual_seed(13)
+    a = torch.tensor([[1.0, 2.0, -1.0, 3.0, -2.0, 1.0, 4.0, -3.0, 2.0]], device="cuda:0", dtype=torch.float16)
+    b = torch.empty(k, n, device="cuda:0", dtype=torch.float16)
+    want = torch.zeros(n, device="cuda:0")
+    for row in range(k):
+        b[row] = torch.randint(-8, 9, (n,), generator=g, device="cuda:0", dtype=torch.int8)
+        want += b[row].float() * float(a[0, row])  # (whole numbers: exact)
+    c = torch.full((n + 3,), 7.0, device="cuda:0", dtype=torch.float16)
+    api.gemmEpilogue(None, 1, n, k, a, b, c, k, n, n)
+    torch.cuda.synchronize()
+    assert torch.equal(c[:n].float(), want) and bool((c[n:] == 7.0).all())
