@@ -484,7 +484,8 @@ def activationGradient(queue, m, n, y, pre, c, y_ld, pre_ld, c_ld, activation="n
 def gemmGrouped(queue, group_count, m, n, k, a, b, c, group_offsets, a_ld, b_ld, c_ld, b_stride, alpha=1.0, beta=0.0,
                 b_transp=False, bias=None, bias_stride=None, activation="none", pre=None, pre_ld=0, a_offset=0, b_offset=0,
                 c_offset=0, bias_offset=0, pre_offset=0, group_offsets_offset=0):
-    """For the rows group_offsets[g] .. group_offsets[g + 1] - 1 of a, c and pre: c = act(alpha a op(b[g]) + bias[g]) + beta c."""
+    """For the rows group_offsets[g] .. group_offsets[g + 1] - 1 of a, c and pre: c = act(alpha a op(b[g]) + bias[g]) + beta c.
+    A `b_stride` or `bias_stride` of 0 is one matrix or bias for all groups; None: one bias behind the other."""
     _layer("gemmGrouped", queue, (a, b, c, bias, pre), group_offsets, (
         TRANS_YES if b_transp else TRANS_NO, m, n, k, alpha, a.data_ptr(), a_offset, a_ld, b.data_ptr(), b_offset, b_ld, b_stride,
         _ptr(bias), bias_offset, n if bias_stride is None else bias_stride, _activation(activation), _ptr(pre), pre_offset, pre_ld,

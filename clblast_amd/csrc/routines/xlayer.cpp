@@ -67,8 +67,9 @@ void TestC(const size_t rows, const size_t cols, const LayerMatrix& matrix, cons
            const size_t stride = 0) {
   TestMatrix(rows, cols, matrix, element, StatusCode::kInvalidLeadDimC, StatusCode::kInsufficientMemoryC, StatusCode::kInvalidMatrixC, count, stride);
 }
+// (stride 0: one vector, read for every group. The sums of groups are given their n as a stride.)
 void TestVector(const size_t n, const LayerVector& vector, const size_t count, const size_t element) {
-  if (vector.stride < n && count > 1) { throw BLASError(StatusCode::kInvalidIncrementX, "vectors of the groups overlap"); }
+  if (vector.stride != 0 && vector.stride < n && count > 1) { throw BLASError(StatusCode::kInvalidIncrementX, "vectors of the groups overlap"); }
   TestMatrix(1, n, LayerMatrix{vector.pointer, vector.offset, n}, element, StatusCode::kInvalidIncrementX,
              StatusCode::kInsufficientMemoryX, StatusCode::kInvalidVectorX, count, vector.stride);
 }

@@ -284,9 +284,9 @@ StatusCode ActivationGradient(const size_t m, const size_t n, const void* y_buff
 // belong to groups: group g owns the rows offsets[g] .. offsets[g + 1] - 1, offsets being group_count + 1 ascending 64-bit
 // integers in DEVICE memory (group_offsets, an element offset from there), so a router's counts need not come to the
 // host. A group may be empty. Rows in front of the first and behind the last group are neither read nor written. Matrix g
-// of B starts b_stride elements behind the one before (0: all groups share one), its bias bias_stride elements. Values that
-// do not ascend or lead outside 0 .. m are clamped so that no access leaves the matrices; what C holds then is not specified. m is
-// below 2^26.
+// of B starts b_stride elements behind the one before (0: all groups share one), its bias bias_stride elements (0: likewise, else
+// at least n). Offsets that do not ascend or lead outside 0 .. m are clamped so that no access leaves the matrices; what C holds
+// then is not specified. m is below 2^26.
 template <typename T>
 StatusCode GemmGrouped(const Transpose b_transpose, const size_t m, const size_t n, const size_t k, const float alpha,
                        const void* a_buffer, const size_t a_offset, const size_t a_ld, const void* b_buffer,

@@ -90,10 +90,28 @@ void FarLines() {
   Reach<half>(true, "many rows, not transposed", (size_t{1} << 31) - 1024, 1, 2, false, true);
   Reach<half>(true, "a long depth of few rows and features", 7, 9, (size_t{1} << 31) - 1024, true, false);
 }
+
+// One bias for all groups, as one matrix for all of them: it is only read
+void SharedBias() {
+  const LayerMatrix a{Place(10 * 14 * 2), 0, 14}, b{Place(3 * 14 * 12 * 2), 0, 12}, c{Place(10 * 12 * 2), 0, 12}, nothing{nullptr, 0, 0};
+  const void* bias = Place(12 * 2);
+  const LayerGroups groups{3, Place(4 * 8), 0};
+  const auto call = [&](const StatusCode code, const char* what, const size_t offset, const size_t stride) {
+    Code<half>(code, what, [&](Xlayer<half>& r) {
+      r.DoGemmGrouped(Transpose::kNo, 10, 12, 14, 1.0f, a, b, 14 * 12, LayerVector{bias, offset, stride}, Activation::kNone, nothing, 0.0f, c, groups);
+    });
+  };
+  call(StatusCode::kSuccess, "one bias for all groups", 0, 0);
+  if (last.bias != bias || last.bias_stride != 0) { ++violations; std::printf("VIOLATION the shared bias\n"); }
+  call(StatusCode::kInsufficientMemoryX, "one bias for all groups, short", 1, 0);
+  call(StatusCode::kInvalidIncrementX, "biases that overlap", 0, 11);
+  call(StatusCode::kInsufficientMemoryX, "a bias for every group", 0, 12);
+}
 }  // namespace
 
 int main() {
   FarLines();
+  SharedBias();
   std::printf("launches %d violations %d\n", launches, violations);
   return violations == 0 ? 0 : 1;
 }

@@ -165,3 +165,19 @@ def test_lines_up_to_the_reach_of_32_bits(gpu):
     api.gemmEpilogue(None, 1, n, k, a, b, c, k, n, n)
     torch.cuda.synchronize()
     assert torch.equal(c[:n].float(), want) and bool((c[n:] == 7.0).all())
+
+
+@pytest.mark.parametrize("dtype", (torch.bfloat16, torch.float16, torch.float32))
+def test_one_bias_for_all_groups(gpu, dtype):
+    g = torch.Generator(device="cuda:0").manual_seed(14)
+    m, n, k, groups = 150, 72, 40, 4
+    a, b, bias = (torch.randn(*shape, generator=g, device="cuda:0").to(dtype) for shape in ((m, k), (groups, k, n), (n,)))
+    bounds = [0, 30, 30, 101, 150]
+    offsets = torch.tensor(bounds, device="cuda:0")
+    c = torch.zeros(m, n, dtype=dtype, device="cuda:0")
+    api.gemmGrouped(None, groups, m, n, k, a, b, c, offsets, k, n, n, k * n, bias=bias, bias_stride=0, activation="silu")
+    torch.cuda.synchronize()
+    for e in range(groups):
+        rows = slice(bounds[e], bounds[e + 1])
+        want, bound, _, _ = ref.epilogue(a[rows].double(), b[e].double(), dtype, 1.0, bias.double(), "silu")
+        ref.check(c[rows], want, bound, "group %d" % e)
