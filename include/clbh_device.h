@@ -268,7 +268,7 @@ CLBH_API int clbh_conv_slab(int precision, const clbh_im2col_shape* shape, int k
 // A * B, there is no product, and c may be NULL where only the sums are wanted (with activation none `pre` may be, too).
 // Groups: offsets is a device array of groups + 1 ascending values. By rows: group g owns the rows offsets[g] ..
 // offsets[g+1] - 1 and has A at a + g * a_stride, bias at bias + g * bias_stride, bias_gradient at bias_gradient + g * m;
-// needs b_kcontig. Rows of no group are neither read nor written. By depth: group g owns that range of k, C at c +
+// needs b_kcontig. Rows of no group are not written and have no effect. By depth: group g owns that range of k, C at c +
 // g * c_stride; needs both operands x-contiguous. Values outside 0 .. n (0 .. k) are clamped.
 // All pointers are those of the first element. residual is not read when beta == 0; it may be C itself.
 #define CLBH_TYPE_FP16 16

@@ -282,11 +282,12 @@ StatusCode ActivationGradient(const size_t m, const size_t n, const void* y_buff
 
 // For every group g: Z = alpha * A_g * op(B_g) + bias_g, C_g = act(Z) + beta * C_g. The rows of A (m x k), C and pre (m x n)
 // belong to groups: group g owns the rows offsets[g] .. offsets[g + 1] - 1, offsets being group_count + 1 ascending 64-bit
-// integers in DEVICE memory (group_offsets, an element offset from there), so a router's counts need not come to the
-// host. A group may be empty. Rows in front of the first and behind the last group are neither read nor written. Matrix g
-// of B starts b_stride elements behind the one before (0: all groups share one), its bias bias_stride elements (0: likewise, else
-// at least n). Offsets that do not ascend or lead outside 0 .. m are clamped so that no access leaves the matrices; what C holds
-// then is not specified. m is below 2^26.
+// integers in DEVICE memory (group_offsets, an element offset from there), so a router's counts need not come to the host.
+// Groups may be empty, all of them too, but m may not be zero. Rows in front of the first and behind the last group are not
+// written and have no effect, whatever they hold (a copy of unaligned rows may read them). Matrix g of B starts b_stride
+// elements behind the one before (0: all groups share one), its bias bias_stride elements (0: likewise, else at least n).
+// Offsets that do not ascend or lead outside 0 .. m are clamped so that no access leaves the matrices; what C holds then is
+// not specified. m is below 2^26.
 template <typename T>
 StatusCode GemmGrouped(const Transpose b_transpose, const size_t m, const size_t n, const size_t k, const float alpha,
                        const void* a_buffer, const size_t a_offset, const size_t a_ld, const void* b_buffer,
