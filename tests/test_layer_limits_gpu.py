@@ -1,5 +1,5 @@
 """The layer products at the edges of what they promise: how often a 16-bit result is not the nearest number, the largest
-numbers of rows and features."""
+numbers of rows, features and groups, the longest depths and lines, one bias for all groups, results in the place of an operand."""
 import pytest
 import torch
 
@@ -181,3 +181,46 @@ def test_one_bias_for_all_groups(gpu, dtype):
         rows = slice(bounds[e], bounds[e + 1])
         want, bound, _, _ = ref.epilogue(a[rows].double(), b[e].double(), dtype, 1.0, bias.double(), "silu")
         ref.check(c[rows], want, bound, "group %d" % e)
+
+
+@pytest.mark.parametrize("dtype", (torch.bfloat16, torch.float16, torch.float32))
+def test_the_activations_input_as_the_result(gpu, dtype):
+    """C of the activation's gradient in the place of Z, by two rows of a wavefront in flight and by rows side by side"""
+    g = torch.Generator(device="cuda:0").manual_seed(15)
+    for m, n in ((1, 1), (37, 9), (301, 520), (1030, 64)):
+        y, z = (torch.randn(m, n, generator=g, device="cuda:0").to(dtype) for _ in range(2))
+        want, bound, want_d, d_bound = ref.gradient(y.double(), torch.zeros(m, n, device="cuda:0", dtype=torch.float64), z.double(), "gelu", dtype)
+        sums = torch.zeros(n, dtype=dtype, device="cuda:0")
+        api.activationGradient(None, m, n, y, z, z, n, n, n, "gelu", bias_gradient=sums)
+        torch.cuda.synchronize()
+        ref.check(z, want, bound, "c of %d x %d" % (m, n))
+        ref.check(sums, want_d, d_bound, "sums of %d x %d" % (m, n))
+
+
+def test_the_most_groups(gpu):
+    """65536 groups, most of one row, some of none or of more than a tile, found by offsets that begin inside their buffer"""
+    g = torch.Generator(device="cuda:0").manual_seed(16)
+    groups, n, k = 65536, 8, 16
+    sizes = torch.ones(groups, dtype=torch.int64)
+    sizes[5::7] = 0
+    sizes[100], sizes[40000], sizes[65535] = 300, 65, 129
+    ends = sizes.cumsum(0)
+    m = int(ends[-1]) + 3
+    offsets = torch.cat([torch.tensor([77, 0, 0]), ends]).to("cuda:0")  # (two values in front of the first)
+    owner = torch.repeat_interleave(torch.arange(groups), sizes).to("cuda:0")
+    a = torch.randint(-4, 5, (m, k), generator=g, device="cuda:0").half()
+    b = torch.randint(-4, 5, (groups, k, n), generator=g, device="cuda:0").half()
+    c = torch.full((m, n), 7.0, device="cuda:0", dtype=torch.float16)
+    api.gemmGrouped(None, groups, m, n, k, a, b, c, offsets, k, n, n, k * n, group_offsets_offset=2)
+    grad = torch.full((groups, k, n), 7.0, device="cuda:0", dtype=torch.float16)
+    api.gemmGroupedGradient(None, groups, m, k, n, a, c, grad, offsets, k, n, n, k * n, alpha=0.0625, group_offsets_offset=2)
+    sums = torch.full((groups, n), 7.0, device="cuda:0", dtype=torch.float16)
+    api.activationGradient(None, m, n, c, None, None, n, 0, 0, bias_gradient=sums, group_count=groups, group_offsets=offsets, group_offsets_offset=2)
+    torch.cuda.synchronize()
+    used = m - 3
+    want = (a[:used].float()[:, :, None] * b[owner].float()).sum(1)  # (whole numbers up to 256: exact)
+    assert torch.equal(c[:used].float(), want) and bool((c[used:] == 7.0).all())
+    want_sums = torch.zeros(groups, n, device="cuda:0").index_add_(0, owner, want)
+    assert torch.equal(sums, want_sums.half())
+    outer = a[:used].float()[:, :, None] * want[:, None, :] * 0.0625
+    assert torch.equal(grad, torch.zeros(groups, k, n, device="cuda:0").index_add_(0, owner, outer).half())
