@@ -12,9 +12,12 @@
 // was fitted to exp(y^2) erfc(y) / 2t, y = x / sqrt(2), on 0 .. 9.5 for the smallest largest relative error (weighted least
 // squares with weights that follow the error): 8.4e-8 = 2^-23.5; with the rounded argument of the exponential 4e-7 up to
 // x = 2, 1.4e-6 up to 5, against 4.9e-4 of an fp16 result's rounding (degree five: 5.2e-6, and one result in 200 rounded
-// the wrong way). The two products more than degree five has are paid for by the clamp that stands where a comparison and a
-// selection stood: GELU's gradient of 8192 x 8192 with the bias's 78.3 -> 78.0 us, 4096 x 8192 x 2048 through it 140.9 -> 140.3,
-// 8192 x 8192 x 4096 with GELU and Z 468.3 -> 470.0. The other form, for fp32 results, calls the math library.
+// the wrong way). The two products more than degree five cost 8192 x 8192 x 4096 with GELU and Z 468 -> 471 us, nothing where
+// memory or another rate is the bound: GELU's gradient of 8192 x 8192 with the bias's 78.3 -> 78.0 us, 4096 x 8192 x 2048 through
+// it 140.9 -> 140.3 (a clamp stands where a comparison and a selection stood). Tried on a card where the former takes 473.1
+// with degree five and 477.7 with seven: degree six (7.4e-7) 476.2, two halves of the polynomial side by side 480.2; a
+// polynomial of degree seven without the factor t (2.5e-7) saves a product and no time, with 2.5 times as many results rounded the
+// wrong way. The other form, for fp32 results, calls the math library.
 // =================================================================================================
 #ifndef CLBLAST_HIP_KERNELS_ACTIVATIONS_HPP_
 #define CLBLAST_HIP_KERNELS_ACTIVATIONS_HPP_

@@ -26,11 +26,11 @@
 // Only the final value is rounded.
 //
 // What bounds it (bf16 and fp32, with the host's time per call where that is part of it): 8192 x 8192 x 4096 with bias, GELU and
-// stored Z 465 us, 1.18 PFLOP/s of the 1.29 that a large library product reaches here - the matrix pipe, and 4 us per
+// stored Z 471 us, 1.17 PFLOP/s of the 1.29 that a large library product reaches here - the matrix pipe, and 4 us per
 // round of tiles for an epilogue under which nothing multiplies (a persistent form that loads the next tile under it held
-// both tiles' registers and was slower, 482 us). fp32 1024 x 1024 x 4096 74 us, 116 of 154 TFLOP/s: the matrix pipe is busy for 74 to
-// 80 % of the cycles, the rest is a barrier per slab of 64 products of a block. Products of few rows: the weights' way from
-// memory, 128 rows over 64 experts of 2048 x 1024 in bf16 42 us for the 205 MB of the experts that have rows. Small ones: the latency of a slab, about 0.15 us, times their number.
+// both tiles' registers and was slower, 482 us). fp32 1024 x 1024 x 4096 74 us, 116 of 154 TFLOP/s: the matrix pipe is busy for 76 %
+// of the cycles, the rest is a barrier per slab of 64 products of a block. Products of few rows: the weights' way from
+// memory, 128 rows over 64 experts of 2048 x 1024 in bf16 41 us for the 205 MB of the experts that have rows. Small ones: the latency of a slab, about 0.15 us, times their number.
 //
 // Teams: few tiles of a long depth leave one work-group to a compute unit, whose four wavefronts wait for each slab. Two sets of
 // wavefronts with half the depth each, in one work-group, halve the number of slabs without a second kernel: 512 x 512 x 4096

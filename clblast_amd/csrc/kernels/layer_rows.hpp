@@ -3,7 +3,7 @@
 //   * LayerRowsKernel: the epilogue of kernels/layer_gemm.hpp on sums that are already there - the fp32 sums of a product
 //     whose K range was split over several work-groups (added up here in the order of the ranges), or, for the gradient of
 //     an activation, a matrix of the caller's. One pass over memory; bound by it: GELU's gradient of 8192 x 8192 bf16 in
-//     72 us, 5.6 TB/s, the rate of a large copy (with one row in flight per wavefront 94, with four 231 - the compiler then spills -
+//     72 us, 5.6 TB/s, the rate of a large copy; with the bias's gradient, whose sums take a second launch, 78 (with one row in flight per wavefront 94, with four 231 - the compiler then spills -
 //     with the matrices kept in the caches 87, with one register more than the 64 that eight wavefronts per SIMD leave 88).
 //   * LayerAlignKernel: copies of operands whose lines do not start at dwords, for the tiled kernel's loads.
 //   * LayerColumnSumsKernel: the second half of a bias gradient, which adds up the sums that the work-groups of either
