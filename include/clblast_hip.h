@@ -240,10 +240,10 @@ StatusCode Convgemm(const KernelMode kernel_mode, const size_t channels, const s
 // matrices are row-major (a column-major caller exchanges A and B, and m and n); offsets, leading dimensions and strides
 // are in elements. The reference has no such routines. Zero sizes return kInvalidDimension, a group count of zero kInvalidBatchCount;
 // the codes of `pre` and `residual` are those of matrix C, the codes of `bias` and `bias_gradient` those of vector X, the
-// codes of `group_offsets` those of vector Y. Sizes are at most 2^31 - 1024, groups at most 65536. Rows of an operand that is
-// multiplied along them are shorter than 2^27 elements (float: 2^26) where it has 16 or more, shorter than 2^28 (2^27) where it is
-// multiplied across them; longer ones return kInvalidDimension. What is written overlaps neither other results nor operands, but
-// for the places that say so.
+// codes of `group_offsets` those of vector Y. Sizes are at most 2^31 - 1024, groups at most 65536. Where a
+// product runs along the rows of an operand (A as it is, B transposed), 15 of its rows, or all but one if there are fewer, take
+// less than 2^32 - 512 bytes without padding, where it runs across them 7 rows do; longer ones return kInvalidDimension. What is
+// written overlaps neither other results nor operands, but for the places that say so.
 
 // Z = alpha * op(A) * op(B) + bias, C = act(Z) + beta * R, for op(A) m x k, op(B) k x n and a bias of n values that every row
 // gets (nullptr: none). Z (m x n) is stored at `pre` as well unless that is nullptr; activation kNone makes this a

@@ -9,6 +9,13 @@ from tests import layer_reference as ref
 pytestmark = pytest.mark.gpu
 
 
+@pytest.fixture(autouse=True)
+def nothing_kept():
+    """The largest of these tests hold 100 GB: what torch keeps of it goes back after each"""
+    yield
+    torch.cuda.empty_cache()
+
+
 def nearest(value, dtype):
     """A 64-bit value rounded once. (The way over 32 bits rounds twice: it only matters within 2^-24 of a border, far less than the
     errors that are counted here.)"""
